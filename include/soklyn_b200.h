@@ -36,7 +36,8 @@ enum {
     SK_ERR_NULL_POINTER = 9,           /* no counterpart: a required pointer is NULL */
     SK_ERR_WORKSPACE = 10,             /* no counterpart: scratch workspace too small */
     SK_ERR_DEVICE_TIMEOUT = 11,        /* no counterpart: a bounded device-side wait gave up */
-    SK_ERR_STATIC_LIMIT = 12           /* no counterpart: size beyond the built-in scratch of sk_column_sums_static */
+    SK_ERR_STATIC_LIMIT = 12,          /* no counterpart: size beyond the built-in scratch of sk_column_sums_static */
+    SK_ERR_INDEX_RANGE = 13            /* no counterpart: a label, class index or sequence offset that a kernel found out of range */
 };
 
 enum { SK_F32 = 0, SK_F16 = 1, SK_BF16 = 2 };
@@ -46,6 +47,7 @@ enum { SK_NORM_DISABLED = 0, SK_NORM_RMS = 1, SK_NORM_LAYER = 2, SK_NORM_BATCH =
 enum { SK_OPT_SGD = 0, SK_OPT_ADAM = 1 };
 enum { SK_REGU_NONE = 0, SK_REGU_L1 = 1, SK_REGU_L2 = 2 };
 enum { SK_LOSS_MSE = 0, SK_LOSS_CROSS_ENTROPY = 1, SK_LOSS_BINARY_CROSS_ENTROPY = 2 };
+enum { SK_PREFERENCE_SIGMOID = 0, SK_PREFERENCE_HINGE = 1, SK_PREFERENCE_SQUARED = 2 };
 
 typedef struct sk_ctx sk_ctx;
 
@@ -134,7 +136,8 @@ int sk_ctx_set_option(sk_ctx *ctx, uint32_t option, uint32_t value);
 /* Grow the scratch workspace; never called implicitly. */
 int sk_ctx_reserve(sk_ctx *ctx, size_t workspace_bytes);
 /* CudaStream::synchronize as called after every launch in src/io/device/ffn_device.rs:75,110,136.
- * Also reports SK_ERR_DEVICE_TIMEOUT if a tensor-core kernel abandoned a bounded wait. */
+ * Also reports SK_ERR_DEVICE_TIMEOUT if a tensor-core kernel abandoned a bounded wait, and SK_ERR_INDEX_RANGE if a loss
+ * (sk_label_logprob and what follows it) met an index out of range since the last call. */
 int sk_sync(sk_ctx *ctx);
 /* Text for a status code, and the detail of the last failure on this context. */
 const char *sk_status_string(int status);
@@ -163,6 +166,10 @@ int sk_step_begin(sk_ctx *ctx, uint32_t slot);
 int sk_step_end(sk_ctx *ctx);
 int sk_step_abort(sk_ctx *ctx);
 int sk_step_stats(const sk_ctx *ctx, uint64_t out[4]);
+/* A host that allocates device memory while a step is being recorded (cudaMalloc is refused then) brackets the
+ * allocation with allow = 1 and allow = 0, on the thread that records. What it allocates has to live until the step has
+ * been launched. Does nothing outside a recorded step. */
+int sk_step_allocations(sk_ctx *ctx, int allow);
 
 /* Per-kernel-class device timing (no counterpart; the reference times phases on the host,
  * examples/mnist_train.rs:180-195). While enabled, every launch of the classes below is
@@ -202,6 +209,95 @@ int sk_dense_forward_batchnorm(sk_ctx *ctx, const sk_dense *layer, const void *x
 int sk_output_error(sk_ctx *ctx, const sk_dense *layer, const void *target, uint32_t target_rows,
                     uint32_t rows, uint32_t loss, uint32_t act, float leaky_coeff);
 
+/* Losses over rows of logits (no counterpart: the reference's losses compare whole output rows with target rows). The
+ * logits are T [rows x cols], typically the `out` of an output block without normalisation, activation and dropout; the
+ * first `classes` columns (0: all) are classes, the others are not read. With z = x / temperature a call takes
+ * log p = log softmax(z) over the classes, writes its losses (f32, one per row or pair, not averaged) and, where
+ * d_logits is given, the gradient of their sum times grad_scale with respect to x, T [rows x cols], zero in the columns
+ * that are no classes. d_logits may be `logits` itself; another overlap is refused. Any row pitch and any base aligned to
+ * an element is taken; rows whose pitch is no multiple of 16 bytes cost a little more, and a gradient that does not lie
+ * on the same offset within 16 bytes as its logits is stored element by element.
+ * Rows that do not count (a label below 0, a weight of 0, no class above -inf) get losses, log-probabilities and
+ * gradients of zero, whatever they hold; a class at -inf has probability 0; a NaN or +inf makes NaN of its own row.
+ * A label or class index at or above `classes` is treated as one below 0 and reported by the next sk_sync
+ * (SK_ERR_INDEX_RANGE). Sums and statistics are f32, sums over a sequence f64. rows = 0 is a call without work. Nothing
+ * is kept between calls and the context's workspace is not used. Results repeat bit for bit. */
+typedef struct {
+    uint32_t dtype;                 /* SK_F32 / SK_F16 / SK_BF16: logits and d_logits */
+    uint32_t rows, cols, classes;
+    const void *logits;
+    void *d_logits;                 /* NULL: no gradient */
+    float temperature;              /* 1e-4 to 1e4 */
+    float grad_scale;               /* factor on the gradient, not on the losses (16-bit gradients: 32 keeps small
+                                       probabilities out of f16's denormals); sk_output_gradient divides by it */
+} sk_logits;
+
+/* logp[row] = log p of labels[row] and, where `entropy` is given, entropy[row] = -sum p log p. d_logits is not used. */
+int sk_label_logprob(sk_ctx *ctx, const sk_logits *logits, const int32_t *labels, float *logp, float *entropy);
+/* Its backward pass: d_logits from the gradients d_logp[row] of the log-probabilities and, where given, d_entropy[row]
+ * of the entropies: (d_logp (1[j = label] - p_j) - d_entropy p_j (log p_j + H)) grad_scale / temperature. */
+int sk_label_logprob_backward(sk_ctx *ctx, const sk_logits *logits, const int32_t *labels, const float *d_logp,
+                              const float *d_entropy);
+
+/* Distillation from a teacher's top logits: k (class, logit) pairs per row, in any order; entries with an index below 0
+ * are unused, an index given twice adds up at its class. Without `lse` the teacher's distribution q is the softmax of
+ * values / temperature over the list and loss = w T^2 sum q (log q - log p). With `lse` (log-sum-exp of the teacher's
+ * logits / temperature over ALL its classes) q = exp(values / temperature - lse), and the mass r = 1 - sum q outside the
+ * list, where it is above 1e-6, is compared with the student's mass outside it: + r (log r - log S). A row with an empty
+ * list and no lse does not count. weights: f32 per row, NULL = 1. k <= 512, classes <= 2^20. */
+typedef struct {
+    const int32_t *indices;         /* [rows x k] */
+    const void *values;             /* values_dtype [rows x k] */
+    uint32_t values_dtype, k;
+    const float *lse, *weights;     /* [rows] or NULL */
+    float *loss;                    /* [rows] */
+} sk_distill;
+int sk_distill_loss(sk_ctx *ctx, const sk_logits *logits, const sk_distill *teacher);
+
+/* Clipped policy loss: ratio = exp(log p(action) - logp_old),
+ *   loss = w (-min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coeff kl - entropy_coeff H),
+ *   kl = exp(d) - d - 1 with d = logp_ref - log p(action).
+ * logp_ref may be NULL where kl_coeff is 0 (kl is 0 then). */
+typedef struct {
+    const int32_t *actions;                     /* [rows] */
+    const float *logp_old, *advantages;         /* [rows] */
+    const float *logp_ref, *weights;            /* [rows] or NULL */
+    float clip_low, clip_high, kl_coeff, entropy_coeff;
+    float *loss, *logp, *kl;                    /* [rows] */
+    float *entropy;                             /* [rows] or NULL */
+} sk_policy;
+int sk_policy_loss(sk_ctx *ctx, const sk_logits *logits, const sk_policy *policy);
+
+/* Preference loss over pairs of packed sequences: sequence s is rows [offsets[s], offsets[s + 1]), 0 <= s < 2 pairs,
+ * sequence 2i the preferred one of pair i and 2i + 1 the other. Lengths may be zero. S = sum of log p(label) over a
+ * sequence's rows that count (`average`: their mean, 0 without any), h = (S_2i - ref_2i) - (S_2i+1 - ref_2i+1),
+ * margin = beta h - target_margin, and with e = label_smoothing
+ *   SIGMOID  loss = w (-(1 - e) log sigmoid(margin) - e log sigmoid(-margin))
+ *   HINGE    loss = w max(0, 1 - margin)
+ *   SQUARED  loss = w (margin - 1/2)^2
+ * Rows below offsets[0] and from offsets[2 pairs] on belong to no sequence: log-probability and gradient zero. Offsets
+ * that fall, or leave [0, rows], make their sequence an empty one and are reported by the next sk_sync. */
+typedef struct {
+    const int32_t *labels;          /* [rows] */
+    const int32_t *offsets;         /* [2 pairs + 1] */
+    uint32_t pairs, form, average;
+    const float *logp_ref;          /* [2 pairs] or NULL (zeros) */
+    const float *weights;           /* [pairs] or NULL */
+    float beta, label_smoothing, target_margin;
+    float *loss, *margin;           /* [pairs] */
+    float *logp;                    /* [2 pairs]: S */
+    float *row_logp;                /* [rows] */
+    float *scratch;                 /* [4 x rows], 16-byte aligned */
+} sk_preference;
+int sk_preference_loss(sk_ctx *ctx, const sk_logits *logits, const sk_preference *preference);
+
+/* Delta of an output block from a gradient of its output that the caller has (one of the losses above, or the
+ * caller's own), in place of sk_output_error: d_out is T [d_rows x N], the gradient times grad_scale; its first `rows`
+ * rows are used. Activation derivative, dropout mask and normalisation backward as sk_hidden_error applies them, with
+ * batch_stat as there. sk_backward_update follows; it divides by its batch, as with the other losses. */
+int sk_output_gradient(sk_ctx *ctx, const sk_dense *layer, const void *d_out, uint32_t d_rows, uint32_t rows,
+                       uint32_t batch_stat, float grad_scale);
+
 /* First half of GpuContext::gpu_hidden_layer_backward_pass (src/io/device/ffn_device.rs:360-436):
  * delta of `cur` from next.d_prenorm and next's (already updated) weights. batch_stat is the
  * batch size used for BatchNorm's 1/M (the whole batch under data parallelism). */
@@ -226,6 +322,11 @@ int sk_ffn_backward(sk_ctx *ctx, const sk_dense *const *layers, uint32_t n_layer
                     uint32_t target_rows, const void *x, uint32_t x_rows, uint32_t loss, uint32_t loss_act,
                     float loss_leaky, const sk_optim *linear, const sk_optim *norm_opt, uint32_t batch,
                     float learn_rate, float grad_clamp, uint32_t step);
+
+/* sk_ffn_backward with sk_output_gradient in place of sk_output_error (no counterpart in the reference). */
+int sk_ffn_backward_gradient(sk_ctx *ctx, const sk_dense *const *layers, uint32_t n_layers, const void *d_out,
+                             uint32_t d_rows, float grad_scale, const void *x, uint32_t x_rows, const sk_optim *linear,
+                             const sk_optim *norm_opt, uint32_t batch, float learn_rate, float grad_clamp, uint32_t step);
 
 /* The two halves of sk_backward_update, for data parallelism (no counterpart in the
  * reference, which is single-device): sk_backward_grads writes the raw batch sums

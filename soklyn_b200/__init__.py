@@ -8,6 +8,8 @@ from .ffn import FeedForwardNetwork
 from .function import (Activation, InitHeNormalFunc, InitHeUniformFunc, InitXavierNormalFunc,
                        InitXavierUniformFunc, InitZeroFunc, LossFunc, Normalisation, Optimiser, Precision,
                        Regularisation)
+from .losses import (DistillLossConfig, PolicyLossConfig, PreferenceForm, PreferenceLossConfig, distill_loss, label_logprob,
+                     label_logprob_backward, policy_loss, preference_loss)
 from .mlp import DenseBlock, ParamState
 from .scheduler import CosineDecayLR, ExponentialLR, ReduceLROnPlateauScheduler, SchedulerMode
 from . import log

@@ -25,7 +25,7 @@ STATUS = {
     0: "ok", 1: "DriverError", 2: "MismatchedDimensions", 3: "AllocationLimitExceeded",
     4: "InvalidConfiguration", 5: "InvalidBatchSize", 6: "TrainingModeRequired",
     7: "HardwareConstraintViolation", 8: "UnsupportedTypeCast", 9: "NullPointer",
-    10: "WorkspaceTooSmall", 11: "DeviceTimeout", 12: "StaticScratchLimit",
+    10: "WorkspaceTooSmall", 11: "DeviceTimeout", 12: "StaticScratchLimit", 13: "IndexRange",
 }
 
 
@@ -53,6 +53,28 @@ class SkExchange(C.Structure):
     """Per-layer pointer tables of sk_dp_backward: arrays of `world` device pointers, one per rank."""
     _fields_ = [("peer_grad", C.c_void_p), ("peer_w", C.c_void_p), ("peer_flags", C.c_void_p), ("peer_colsums", C.c_void_p),
                 ("mc_grad", C.c_void_p), ("mc_w", C.c_void_p)]
+
+
+class SkLogits(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("cols", C.c_uint32), ("classes", C.c_uint32),
+                ("logits", C.c_void_p), ("d_logits", C.c_void_p), ("temperature", C.c_float), ("grad_scale", C.c_float)]
+
+
+class SkDistill(C.Structure):
+    _fields_ = [("indices", C.c_void_p), ("values", C.c_void_p), ("values_dtype", C.c_uint32), ("k", C.c_uint32),
+                ("lse", C.c_void_p), ("weights", C.c_void_p), ("loss", C.c_void_p)]
+
+
+class SkPolicy(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("actions", "logp_old", "advantages", "logp_ref", "weights")]
+                + [(n, C.c_float) for n in ("clip_low", "clip_high", "kl_coeff", "entropy_coeff")]
+                + [(n, C.c_void_p) for n in ("loss", "logp", "kl", "entropy")])
+
+
+class SkPreference(C.Structure):
+    _fields_ = ([("labels", C.c_void_p), ("offsets", C.c_void_p), ("pairs", C.c_uint32), ("form", C.c_uint32), ("average", C.c_uint32),
+                 ("logp_ref", C.c_void_p), ("weights", C.c_void_p), ("beta", C.c_float), ("label_smoothing", C.c_float),
+                 ("target_margin", C.c_float)] + [(n, C.c_void_p) for n in ("loss", "margin", "logp", "row_logp", "scratch")])
 
 
 def sources() -> list[str]:
@@ -108,6 +130,7 @@ _SIGS = {
     "sk_step_end": (C.c_int, [C.c_void_p]),
     "sk_step_abort": (C.c_int, [C.c_void_p]),
     "sk_step_stats": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "sk_step_allocations": (C.c_int, [C.c_void_p, C.c_int]),
     "sk_profile_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "sk_profile_read": (C.c_int, [C.c_void_p, C.c_uint32, C.POINTER(C.c_uint64), C.POINTER(C.c_double)]),
     "sk_scramble_seed": (C.c_uint32, [C.c_uint32, C.c_uint32]),
@@ -117,6 +140,12 @@ _SIGS = {
                                              C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32]),
     "sk_output_error": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32,
                                   C.c_uint32, C.c_uint32, C.c_float]),
+    "sk_label_logprob": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_label_logprob_backward": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkDistill)]),
+    "sk_policy_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkPolicy)]),
+    "sk_preference_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkPreference)]),
+    "sk_output_gradient": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float]),
     "sk_hidden_error": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.POINTER(SkDense), C.c_uint32, C.c_uint32]),
     "sk_backward_update": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32,
                                      C.POINTER(SkOptim), C.POINTER(SkOptim), C.c_float, C.c_float, C.c_uint32]),
@@ -125,6 +154,8 @@ _SIGS = {
     "sk_ffn_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32,
                                   C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_void_p, C.c_uint32, C.c_float,
                                   C.c_float, C.c_uint32]),
+    "sk_ffn_backward_gradient": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint32, C.c_float, C.c_void_p,
+                                           C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_float, C.c_float, C.c_uint32]),
     "sk_backward_grads": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32,
                                     C.c_void_p, C.c_void_p]),
     "sk_apply_update": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_void_p, C.c_uint32,

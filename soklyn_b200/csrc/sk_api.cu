@@ -15,60 +15,11 @@
 #include <map>
 #include <tuple>
 
+#include "sk_context.cuh"
 #include "sk_gemm_simt.cuh"
 #include "sk_exchange.cuh"
 #include "sk_gemm_tc.cuh"
 #include "sk_rowwise.cuh"
-
-struct sk_ctx {
-    int device = 0;
-    uint32_t tile_dim = 16;
-    cudaStream_t stream = nullptr;
-    bool own_stream = false;
-    void *workspace = nullptr;
-    size_t workspace_bytes = 0;
-    int num_sms = 148;
-    size_t smem_optin = 0;
-    uint64_t launches = 0;
-    char err[512] = {0};
-    // tensor-core path
-    int cc_major = 0;
-    uint32_t gemm_engine = 0;              // 0 auto, 1 FFMA only
-    int *tc_err = nullptr;                 // device word a tcgen05 kernel sets when a bounded wait gives up
-    void *encode_tiled = nullptr;          // cuTensorMapEncodeTiled, resolved through the runtime
-    std::map<std::tuple<const void *, uint64_t, uint64_t, uint64_t, uint32_t, uint32_t>, CUtensorMap> tmaps;
-    uint64_t tc_launches = 0;
-    uint32_t tc_group_n = 8;               // tile columns walked together (SK_TC_GROUP_N at context creation)
-    uint32_t handover_min_rows = 0;        // column sums ride in the dX epilogue from this many rows on (SK_HANDOVER_MIN_ROWS at context creation)
-    uint32_t reserve_sms = 0;              // SMs the tensor-core GEMMs leave free (for a concurrent exchange kernel)
-    uint32_t cluster_blocks[4] = {0, 0, 0, 0};   // blocks the chip holds at once in clusters of 1, 2, 4, 8 (one block per SM; 0: none)
-    bool lean = false;                     // SK_OPTION_LEAN_BACKWARD
-    // data-parallel backward
-    uint32_t *dp_counters = nullptr;       // one completion counter per (layer, block), zero between launches
-    // f32 GEMMs on the tensor cores (SK_OPTION_F32_TENSOR_CORES): device copies of the tensor maps of a launch
-    bool f32_tensor = false;
-    sk::TcSplitMaps *split_maps = nullptr; // ring of kSplitMapSlots entries
-    uint32_t split_slot = 0;
-    // Column sums handed from the dX epilogue to the weight update of the same layer. Only inside
-    // sk_ffn_backward (nothing can touch the tensors or the workspace in between there).
-    bool in_ffn_backward = false;
-    bool colsum_handover = false;             // SK_OPTION_COLSUM_HANDOVER
-    const void *fused_colsum_key = nullptr;   // d_prenorm of the layer whose partial sums sit in the workspace
-    uint32_t fused_colsum_groups = 0, fused_colsum_batch = 0;
-    // whole-step graphs (sk_step_begin / sk_step_end)
-    struct StepGraph { cudaGraphExec_t exec = nullptr; bool warmed = false; };
-    StepGraph step_graphs[SK_STEP_SLOTS];
-    int step_open = -1;                    // slot between begin and end
-    bool step_capturing = false;
-    cudaStream_t record_stream = nullptr;  // the calls of a step are recorded on this stream (the legacy default stream
-    cudaStream_t user_stream = nullptr;    // cannot be captured); `stream` points here meanwhile, user_stream keeps the caller's
-    uint64_t step_stats[4] = {0, 0, 0, 0}; // instantiated, updated in place, launched, unrecorded steps
-    // optional per-class event timing
-    bool profiling = false;
-    std::vector<cudaEvent_t> ev_pool;      // pairs: [2i] start, [2i+1] stop
-    std::vector<uint32_t> ev_class;        // class of pair i
-    size_t ev_used = 0;
-};
 
 namespace {
 using namespace sk;
@@ -76,44 +27,6 @@ using namespace sk;
 constexpr uint32_t kSplitMapSlots = 16;
 constexpr uint32_t kDpMaxLayers = 64;
 constexpr uint32_t kDpCounterWords = kDpMaxLayers * kMaxChunks;
-
-int fail(sk_ctx *c, int code, const char *fmt, ...) {
-    if (c) {
-        va_list ap;
-        va_start(ap, fmt);
-        vsnprintf(c->err, sizeof c->err, fmt, ap);
-        va_end(ap);
-    }
-    return code;
-}
-
-int step_recording(sk_ctx *c) {
-    return fail(c, SK_ERR_INVALID_CONFIGURATION, "not while a step graph is being recorded (sk_step_end or sk_step_abort first)");
-}
-
-int check_cuda(sk_ctx *c, cudaError_t e, const char *what) {
-    if (e == cudaSuccess) return SK_OK;
-    return fail(c, SK_ERR_DRIVER, "%s: %s", what, cudaGetErrorString(e));
-}
-
-// Brackets one launch with events when profiling is on.
-struct ProfScope {
-    sk_ctx *c;
-    size_t slot = (size_t)-1;
-    cudaStream_t st;
-    ProfScope(sk_ctx *ctx, uint32_t cls, cudaStream_t on = nullptr) : c(ctx), st(on ? on : ctx->stream) {
-        if (!c->profiling) return;
-        if (c->ev_used * 2 + 2 > c->ev_pool.size()) {
-            cudaEvent_t a, b;
-            if (cudaEventCreate(&a) != cudaSuccess || cudaEventCreate(&b) != cudaSuccess) return;
-            c->ev_pool.push_back(a); c->ev_pool.push_back(b); c->ev_class.push_back(cls);
-        }
-        slot = c->ev_used++;
-        c->ev_class[slot] = cls;
-        cudaEventRecord(c->ev_pool[2 * slot], st);
-    }
-    ~ProfScope() { if (slot != (size_t)-1) cudaEventRecord(c->ev_pool[2 * slot + 1], st); }
-};
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -592,6 +505,27 @@ int output_error_impl(sk_ctx *c, const sk_dense *L, const void *target, uint32_t
         (T *)L->out, (const T *)L->preact, (const T *)target, (const float *)master_of<T>(L->master_norm_w, L->norm_w), L->grad,
         L->d_prenorm, L->d_norm_w, L->d_norm_b, L->dtype == SK_F32 ? nullptr : (T *)L->d_prenorm_lp,
         (const T *)L->norm_rstd, (const T *)L->centered, (const T *)L->prenorm, rows, L->N, loss, L->norm, act, leaky), "output error");
+}
+
+// Delta of a block from a gradient with respect to its output: what hidden_error_impl does behind its product, with the
+// product replaced by the caller's gradient at the loss scale.
+template <typename T>
+int output_gradient_impl(sk_ctx *c, const sk_dense *L, const void *d_out, uint32_t rows, uint32_t batch_stat, float grad_scale) {
+    EpiHidden<T> epi{};
+    epi.predrop = (const T *)L->predrop; epi.preact = (const T *)L->preact; epi.mask = (const T *)L->mask;
+    epi.prenorm = (const T *)L->prenorm; epi.centered = (const T *)L->centered; epi.rstd = (const T *)L->norm_rstd;
+    epi.norm_w = master_of<T>(L->master_norm_w, L->norm_w);
+    epi.grad = L->grad; epi.d_prenorm = L->d_prenorm; epi.d_norm_w = L->d_norm_w; epi.d_norm_b = L->d_norm_b;
+    epi.d_prenorm_lp = L->dtype == SK_F32 ? nullptr : (T *)L->d_prenorm_lp;
+    epi.N = L->N; epi.norm = L->norm; epi.act = L->act; epi.leaky = L->leaky_coeff;
+    epi.inv_n = 1.0f / (float)L->N; epi.inv_m = 1.0f / (float)batch_stat; epi.vec_ok = layer_vec_ok(L) && aligned16(d_out);
+    epi.acc_scale = kLossScale / grad_scale;
+    const size_t items = (size_t)rows * (epi.vec_ok ? L->N / 8 : L->N);
+    const size_t blocks = std::min((items + kRowThreads - 1) / kRowThreads, (size_t)c->num_sms * 16);
+    ProfScope ps(c, SK_PROF_OUTPUT_ERROR);
+    c->launches++;
+    return check_cuda(c, launch_step(c->stream, overlaps<T>(c), dim3((uint32_t)blocks), kRowThreads, 0, dim3(1), output_gradient_kernel<T>, epi,
+                                     (const T *)d_out, rows), "output gradient");
 }
 
 template <typename T>
@@ -1080,8 +1014,10 @@ int sk_ctx_create(int device, uint32_t tile_dim, void *stream, int create_stream
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
             c->encode_tiled = fn;
-        if (cudaMalloc(&c->tc_err, sizeof(int)) == cudaSuccess) cudaMemset(c->tc_err, 0, sizeof(int));
-        else c->tc_err = nullptr;
+        if (cudaMalloc(&c->tc_err, 2 * sizeof(int)) == cudaSuccess) {
+            cudaMemset(c->tc_err, 0, 2 * sizeof(int));
+            c->loss_err = c->tc_err + 1;
+        } else c->tc_err = nullptr;
         if (cudaMalloc(&c->dp_counters, kDpCounterWords * sizeof(uint32_t)) == cudaSuccess)
             cudaMemset(c->dp_counters, 0, kDpCounterWords * sizeof(uint32_t));
         else c->dp_counters = nullptr;
@@ -1144,13 +1080,15 @@ int sk_sync(sk_ctx *c) {
     if (!c) return SK_ERR_NULL_POINTER;
     if (c->step_capturing) return step_recording(c);
     int rc = check_cuda(c, cudaStreamSynchronize(c->stream), "stream synchronize");
-    if (rc || !c->tc_err || c->tc_launches == 0) return rc;
-    int flag = 0;
-    if ((rc = check_cuda(c, cudaMemcpy(&flag, c->tc_err, sizeof(int), cudaMemcpyDeviceToHost), "error flag read"))) return rc;
-    if (flag != 0) {
-        cudaMemset(c->tc_err, 0, sizeof(int));
-        return fail(c, SK_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (code %d: 1 TMA loader, 2 MMA issuer, 3 GEMM epilogue, 5 peer flags)", flag);
-    }
+    if (rc || !c->tc_err || (c->tc_launches == 0 && c->loss_launches == 0)) return rc;
+    int flag[2] = {0, 0};
+    if ((rc = check_cuda(c, cudaMemcpy(flag, c->tc_err, sizeof flag, cudaMemcpyDeviceToHost), "error flag read"))) return rc;
+    if (flag[0] != 0 || flag[1] != 0) cudaMemset(c->tc_err, 0, sizeof flag);
+    if (flag[0] != 0)
+        return fail(c, SK_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (code %d: 1 TMA loader, 2 MMA issuer, 3 GEMM epilogue, 5 peer flags)", flag[0]);
+    if (flag[1] != 0)
+        return fail(c, SK_ERR_INDEX_RANGE, "out of range since the last sk_sync:%s%s%s", flag[1] & 1 ? " a label" : "", flag[1] & 2 ? " a class of a teacher's list" : "",
+                    flag[1] & 4 ? " a sequence offset" : "");
     return SK_OK;
 }
 
@@ -1230,6 +1168,13 @@ int sk_step_stats(const sk_ctx *c, uint64_t out[4]) {
     return SK_OK;
 }
 
+int sk_step_allocations(sk_ctx *c, int allow) {
+    if (!c) return SK_ERR_NULL_POINTER;
+    if (!c->step_capturing) return SK_OK;
+    cudaStreamCaptureMode mode = allow ? cudaStreamCaptureModeRelaxed : cudaStreamCaptureModeGlobal;   // a thread's mode is global unless changed
+    return check_cuda(c, cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+}
+
 int sk_ctx_set_option(sk_ctx *c, uint32_t option, uint32_t value) {
     if (!c) return SK_ERR_NULL_POINTER;
     if (c->step_capturing) return step_recording(c);
@@ -1259,6 +1204,7 @@ const char *sk_status_string(int s) {
     case SK_ERR_NULL_POINTER: return "Required pointer is NULL";
     case SK_ERR_WORKSPACE: return "Scratch workspace too small";
     case SK_ERR_DEVICE_TIMEOUT: return "Device-side wait timed out";
+    case SK_ERR_INDEX_RANGE: return "Index out of range";
     case SK_ERR_STATIC_LIMIT: return "Size exceeds the built-in scratch array (N may not exceed 262144 columns)";
     default: return "unknown status";
     }
@@ -1351,6 +1297,20 @@ int sk_output_error(sk_ctx *c, const sk_dense *L, const void *target, uint32_t t
     return SK_DISPATCH(L->dtype, output_error_impl, c, L, target, rows, loss, act, leaky);
 }
 
+int sk_output_gradient(sk_ctx *c, const sk_dense *L, const void *d_out, uint32_t d_rows, uint32_t rows, uint32_t batch_stat, float grad_scale) {
+    int rc = check_layer(c, L, true);
+    if (rc) return rc;
+    if (!d_out) return fail(c, SK_ERR_NULL_POINTER, "gradient pointer is NULL");
+    c->fused_colsum_key = nullptr;   // column sums handed over by sk_hidden_error are for the very next call only
+    if (d_rows > L->max_batch) return fail(c, SK_ERR_ALLOCATION_LIMIT, "gradient batches: received %u exceeds max %u", d_rows, L->max_batch);
+    if (rows == 0 || batch_stat == 0) return fail(c, SK_ERR_INVALID_BATCH_SIZE, "Batch size must be more than zero.");
+    if (rows > d_rows) return fail(c, SK_ERR_MISMATCHED_DIMENSIONS, "gradient rows vs explicit batch size: expected %u, found %u", rows, d_rows);
+    if (L->act == SK_ACT_SOFTMAX) return fail(c, SK_ERR_INVALID_CONFIGURATION, "Softmax activation can only be passed into the compute_loss function.");
+    if (L->norm == SK_NORM_BATCH && batch_stat == 1) return fail(c, SK_ERR_INVALID_BATCH_SIZE, "BatchNorm needs a batch size of more than 1.");
+    if (!(std::isfinite(grad_scale) && grad_scale > 0.0f)) return fail(c, SK_ERR_INVALID_CONFIGURATION, "gradient scale %g must be positive", (double)grad_scale);
+    return SK_DISPATCH(L->dtype, output_gradient_impl, c, L, d_out, rows, batch_stat, grad_scale);
+}
+
 int sk_hidden_error(sk_ctx *c, const sk_dense *cur, const sk_dense *next, uint32_t batch, uint32_t batch_stat) {
     int rc = check_layer(c, cur, true);
     if (rc) return rc;
@@ -1397,13 +1357,9 @@ int sk_ffn_forward(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const v
     return SK_OK;
 }
 
-int sk_ffn_backward(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const void *target, uint32_t target_rows,
-                    const void *x, uint32_t x_rows, uint32_t loss, uint32_t loss_act, float loss_leaky,
-                    const sk_optim *lin, const sk_optim *nrm, uint32_t batch, float lr, float clamp, uint32_t step) {
-    if (!c || !layers || !lin || !nrm) return SK_ERR_NULL_POINTER;
-    if (n == 0) return fail(c, SK_ERR_INVALID_CONFIGURATION, "Backward pass on an empty network");
-    for (uint32_t i = 0; i < n; ++i)
-        if (!layers[i]) return fail(c, SK_ERR_NULL_POINTER, "layer %u is NULL", i);
+// The updates of all blocks behind the output block's delta, and the hidden deltas between them.
+static int ffn_updates(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const void *x, uint32_t x_rows, const sk_optim *lin,
+                       const sk_optim *nrm, uint32_t batch, float lr, float clamp, uint32_t step) {
     const uint32_t last = n - 1;
     auto input_of = [&](uint32_t i, uint32_t &rows) -> const void * {
         if (i == 0) { rows = x_rows; return x; }
@@ -1411,10 +1367,8 @@ int sk_ffn_backward(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const 
         return layers[i - 1]->out;
     };
     uint32_t rows = 0;
-    int rc = sk_output_error(c, layers[last], target, target_rows, layers[last]->max_batch, loss, loss_act, loss_leaky);
-    if (rc) return rc;
     const void *in = input_of(last, rows);
-    if ((rc = sk_backward_update(c, layers[last], in, rows, batch, &lin[last], &nrm[last], lr, clamp, step))) return rc;
+    int rc = sk_backward_update(c, layers[last], in, rows, batch, &lin[last], &nrm[last], lr, clamp, step);
     for (uint32_t i = last; i-- > 0 && rc == SK_OK;) {
         c->in_ffn_backward = true;    // the update of layer i follows its delta directly: sums may be handed over
         rc = sk_hidden_error(c, layers[i], layers[i + 1], batch, batch);
@@ -1425,6 +1379,32 @@ int sk_ffn_backward(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const 
     }
     c->fused_colsum_key = nullptr;
     return rc;
+}
+
+static int check_stack(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const sk_optim *lin, const sk_optim *nrm) {
+    if (!c || !layers || !lin || !nrm) return SK_ERR_NULL_POINTER;
+    if (n == 0) return fail(c, SK_ERR_INVALID_CONFIGURATION, "Backward pass on an empty network");
+    for (uint32_t i = 0; i < n; ++i)
+        if (!layers[i]) return fail(c, SK_ERR_NULL_POINTER, "layer %u is NULL", i);
+    return SK_OK;
+}
+
+int sk_ffn_backward(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const void *target, uint32_t target_rows,
+                    const void *x, uint32_t x_rows, uint32_t loss, uint32_t loss_act, float loss_leaky,
+                    const sk_optim *lin, const sk_optim *nrm, uint32_t batch, float lr, float clamp, uint32_t step) {
+    int rc = check_stack(c, layers, n, lin, nrm);
+    if (rc) return rc;
+    if ((rc = sk_output_error(c, layers[n - 1], target, target_rows, layers[n - 1]->max_batch, loss, loss_act, loss_leaky))) return rc;
+    return ffn_updates(c, layers, n, x, x_rows, lin, nrm, batch, lr, clamp, step);
+}
+
+int sk_ffn_backward_gradient(sk_ctx *c, const sk_dense *const *layers, uint32_t n, const void *d_out, uint32_t d_rows, float grad_scale,
+                             const void *x, uint32_t x_rows, const sk_optim *lin, const sk_optim *nrm, uint32_t batch, float lr,
+                             float clamp, uint32_t step) {
+    int rc = check_stack(c, layers, n, lin, nrm);
+    if (rc) return rc;
+    if ((rc = sk_output_gradient(c, layers[n - 1], d_out, d_rows, batch, batch, grad_scale))) return rc;
+    return ffn_updates(c, layers, n, x, x_rows, lin, nrm, batch, lr, clamp, step);
 }
 
 int sk_backward_grads(sk_ctx *c, const sk_dense *L, const void *x, uint32_t x_rows, uint32_t batch, float *dw,

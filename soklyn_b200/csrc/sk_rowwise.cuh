@@ -420,6 +420,27 @@ output_error_elem_kernel(const T *__restrict__ out, const T *__restrict__ preact
     }
 }
 
+// A block's delta from a gradient with respect to its output: the epilogue of the dX product (EpiHidden) on values that
+// the caller has. Element-wise, 8 elements per thread where the tensors allow 128-bit accesses.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+output_gradient_kernel(EpiHidden<T> epi, const T *__restrict__ d_out, uint32_t M) {
+    constexpr int V = 8;
+    grid_ready();
+    const size_t stride = (size_t)gridDim.x * blockDim.x, at = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint32_t per_row = epi.vec_ok ? epi.N / V : epi.N;
+    for (size_t i = at; i < (size_t)M * per_row; i += stride) {
+        const uint32_t row = (uint32_t)(i / per_row), col = (uint32_t)(i % per_row) * (epi.vec_ok ? V : 1);
+        if (epi.vec_ok) {
+            float d[V];
+            load_run<T, V>(d_out + (size_t)row * epi.N + col, true, d);
+            epi.template run<V>(row, col, d, V);
+        } else {
+            epi.one(row, col, to_f32(d_out[(size_t)row * epi.N + col]));
+        }
+    }
+}
+
 // Column sums over the batch of d_prenorm, d_norm_w, d_norm_b (the row-0 work of
 // ffn/backward.cu:181-194). Stage 1: each block sums `rows_per_block` rows of 32 columns
 // into partial[blockIdx.y][which][col]; stage 2 adds the partials in a fixed order.

@@ -13,7 +13,7 @@ import ctypes as C
 import torch
 
 from . import _native, log
-from ._native import SkDense, SkOptim
+from ._native import SkDense, SkDistill, SkLogits, SkOptim, SkPolicy, SkPreference
 from .core import SK_DTYPE, Tensor
 from .function import Activation, LossFunc, Normalisation, Optimiser, Precision
 
@@ -39,6 +39,7 @@ class GpuContext:
         if rc != 0:
             raise log.DriverError(f"sk_ctx_create failed with status {rc} ({_native.STATUS.get(rc)})")
         self.handle = handle
+        self.step_keeps = None   # buffers of calls recorded in an open step graph, which run only when it ends
 
     @staticmethod
     def new(tile_dim: int) -> "GpuContext":
@@ -108,12 +109,43 @@ class GpuContext:
         launch-bound networks. Inside the block nothing may wait for the stream or read a tensor back; the first
         step of a slot runs unrecorded. `slot` names the executable graph that is reused from step to step."""
         self._check(self.lib.sk_step_begin(self.handle, slot))
+        keeps, self.step_keeps = self.step_keeps, []
         try:
-            yield
-        except BaseException:
-            self.lib.sk_step_abort(self.handle)
-            raise
-        self._check(self.lib.sk_step_end(self.handle))
+            try:
+                yield
+            except BaseException:
+                self.lib.sk_step_abort(self.handle)
+                raise
+            self._check(self.lib.sk_step_end(self.handle))
+        finally:
+            self.step_keeps = keeps
+
+    def new_buffer(self, shape, dtype: torch.dtype) -> torch.Tensor:
+        """Uninitialised memory of this context's stream; inside a step graph it is kept until the step has been launched."""
+        if self.step_keeps is not None:
+            self._check(self.lib.sk_step_allocations(self.handle, 1))
+            try:
+                t = self._empty(shape, dtype)
+            finally:
+                self._check(self.lib.sk_step_allocations(self.handle, 0))
+            self.step_keeps.append(t)
+            return t
+        return self._empty(shape, dtype)
+
+    def _empty(self, shape, dtype):
+        if torch.cuda.current_stream(self.device) == self.stream:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def uses(self, tensors):
+        """These tensors are read or written by calls made so far: memory that another stream owns is not handed out
+        again before they are through, and that of a recorded step not before it is launched."""
+        if torch.cuda.current_stream(self.device) != self.stream:
+            for t in tensors:
+                t.record_stream(self.stream)
+        if self.step_keeps is not None:
+            self.step_keeps.extend(tensors)
 
     def step_graph_stats(self) -> dict:
         out = (C.c_uint64 * 4)()
@@ -184,6 +216,27 @@ class GpuContext:
                                                 train_ctx.batch_size, C.byref(lin), C.byref(nrm),
                                                 train_ctx.learn_rate, train_ctx.grad_clamp, step & 0xFFFFFFFF))
 
+    def gpu_output_gradient(self, layer, d_out: Tensor, batch_size: int, grad_scale: float = 1.0, batch_stat: int | None = None):
+        """Delta of an output block from a gradient of its output (times grad_scale), in place of a loss against a target."""
+        self._check(self.lib.sk_output_gradient(self.handle, C.byref(layer.desc()), d_out.ptr(), d_out.rows(), batch_size,
+                                                batch_size if batch_stat is None else batch_stat, grad_scale))
+
+    # -- losses over rows of logits (no counterpart in the reference); arguments are checked by soklyn_b200/losses.py --
+    def gpu_label_logprob(self, logits: SkLogits, labels: int, logp: int, entropy: "int | None"):
+        self._check(self.lib.sk_label_logprob(self.handle, C.byref(logits), labels, logp, entropy))
+
+    def gpu_label_logprob_backward(self, logits: SkLogits, labels: int, d_logp: int, d_entropy: "int | None"):
+        self._check(self.lib.sk_label_logprob_backward(self.handle, C.byref(logits), labels, d_logp, d_entropy))
+
+    def gpu_distill_loss(self, logits: SkLogits, teacher: SkDistill):
+        self._check(self.lib.sk_distill_loss(self.handle, C.byref(logits), C.byref(teacher)))
+
+    def gpu_policy_loss(self, logits: SkLogits, policy: SkPolicy):
+        self._check(self.lib.sk_policy_loss(self.handle, C.byref(logits), C.byref(policy)))
+
+    def gpu_preference_loss(self, logits: SkLogits, preference: SkPreference):
+        self._check(self.lib.sk_preference_loss(self.handle, C.byref(logits), C.byref(preference)))
+
     def gpu_hidden_layer_error(self, cur, nxt, batch_size: int, batch_stat: int | None = None):
         self.check_tile_dim(cur.precision)
         self._check(self.lib.sk_hidden_error(self.handle, C.byref(cur.desc()), C.byref(nxt.desc()), batch_size,
@@ -239,6 +292,15 @@ class GpuContext:
                                              loss_config.loss_func.value, act.ordinal(), act.coeff, lin, nrm,
                                              train_ctx.batch_size, train_ctx.learn_rate, train_ctx.grad_clamp,
                                              step & 0xFFFFFFFF))
+
+    def gpu_ffn_backward_gradient(self, layers, d_out: Tensor, grad_scale: float, input: Tensor, train_ctx, step: int):
+        n = len(layers)
+        ptrs = (C.c_void_p * n)(*[C.addressof(l.desc()) for l in layers])
+        lin = (SkOptim * n)(*[_optim(o) for o in train_ctx.optimisers])
+        nrm = (SkOptim * n)(*[_optim(o) for o in train_ctx.norm_optimisers])
+        self._check(self.lib.sk_ffn_backward_gradient(self.handle, ptrs, n, d_out.ptr(), d_out.rows(), grad_scale, input.ptr(),
+                                                      input.rows(), lin, nrm, train_ctx.batch_size, train_ctx.learn_rate,
+                                                      train_ctx.grad_clamp, step & 0xFFFFFFFF))
 
     # -- data-parallel backward: the whole pass in one native call --
     def dp_blocks(self, k: int, n: int, world: int, wanted: int) -> int:

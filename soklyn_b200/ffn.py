@@ -62,6 +62,28 @@ class FeedForwardNetwork:
             layer_input = outputs[i - 1] if i > 0 else input
             self.layers[i].backward_hidden(context, self.layers[i + 1], layer_input, train_ctx.get_train_context(i), step)
 
+    def backward_gradient(self, context, outputs: Sequence[Tensor], d_out: Tensor, input: Tensor,
+                          train_ctx: MultiLayerTrainContext, step: int, grad_scale: float = 1.0):
+        """`backward` from a gradient of the last block's output (times grad_scale) that the caller has, such as the
+        d_logits of the losses in soklyn_b200/losses.py, in place of a target; no counterpart in the reference. The
+        update divides by the batch size, as it does with the other losses."""
+        n = len(self.layers)
+        if n == 0 or len(outputs) != n or len(train_ctx.optimisers) != n:
+            raise log.InvalidConfiguration(
+                f"Backward pass expects exactly {n} activation vectors and optimizers. "
+                f"Found {len(outputs)} outputs, {len(train_ctx.optimisers)} optimisers.")
+        last = n - 1
+        if callable(getattr(context, "gpu_ffn_backward_gradient", None)) and all(o is l.get_outputs() for o, l in zip(outputs, self.layers)):
+            self.layers[last].check_output_gradient(d_out, train_ctx.batch_size, grad_scale)
+            self._check_layers(input, train_ctx)
+            context.gpu_ffn_backward_gradient(self.layers, d_out, grad_scale, input, train_ctx, step)
+            return
+        self.layers[last].output_gradient(context, d_out, train_ctx.batch_size, grad_scale)
+        self.layers[last].backward_output(context, outputs[last - 1] if last > 0 else input, train_ctx.get_train_context(last), step)
+        for i in range(last - 1, -1, -1):
+            layer_input = outputs[i - 1] if i > 0 else input
+            self.layers[i].backward_hidden(context, self.layers[i + 1], layer_input, train_ctx.get_train_context(i), step)
+
     def _check_backward(self, target, input, loss_config, train_ctx):
         """The host-side checks of compute_loss / backward_output / backward_hidden (src/mlp.rs:607-821)."""
         from .function import Activation, LossFunc
@@ -79,6 +101,11 @@ class FeedForwardNetwork:
             raise log.InvalidConfiguration("Cross-Entropy Loss only supports the Softmax activation function.")
         if lf == LossFunc.BinaryCrossEntropy and act != Activation.Sigmoid:
             raise log.InvalidConfiguration("Binary Cross-Entropy only supports the Sigmoid activation function.")
+        self._check_layers(input, train_ctx)
+
+    def _check_layers(self, input, train_ctx):
+        if not all(l.is_training_mode() for l in self.layers):
+            raise log.TrainingModeRequired("backward pass")
         cur = input
         for i, layer in enumerate(self.layers):
             layer.check_input_dimension(cur, train_ctx.batch_size)

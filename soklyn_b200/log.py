@@ -54,12 +54,16 @@ class UnsupportedTypeCast(Error):
         super().__init__(f"Unsupported precision cast operation: Cannot convert data from {src} to {dst}")
 
 
+class IndexOutOfRange(Error):
+    """A label, class index or sequence offset that a kernel found out of range (no counterpart in the reference)."""
+
+
 class NativeError(Error):
     """A status code of the C ABI that has no counterpart in the reference."""
 
 
 _BY_STATUS = {1: DriverError, 2: MismatchedDimensions, 3: AllocationLimitExceeded, 4: InvalidConfiguration,
-              5: InvalidBatchSize, 6: TrainingModeRequired, 7: HardwareConstraintViolation, 8: UnsupportedTypeCast}
+              5: InvalidBatchSize, 6: TrainingModeRequired, 7: HardwareConstraintViolation, 8: UnsupportedTypeCast, 13: IndexOutOfRange}
 
 
 def raise_status(status: int, detail: str):

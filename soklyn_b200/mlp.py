@@ -273,3 +273,24 @@ class DenseBlock:
         if lf == LossFunc.BinaryCrossEntropy and act != Activation.Sigmoid:
             raise log.InvalidConfiguration("Binary Cross-Entropy only supports the Sigmoid activation function.")
         context.gpu_compute_output_layer_error(self, target, lf, act)
+
+    def output_gradient(self, context, d_out: Tensor, batch_size: int, grad_scale: float = 1.0):
+        """This output block's delta from a gradient of its output (times grad_scale), in place of compute_loss; no
+        counterpart in the reference. backward_output follows."""
+        self.check_output_gradient(d_out, batch_size, grad_scale)
+        context.gpu_output_gradient(self, d_out, batch_size, grad_scale)
+
+    def check_output_gradient(self, d_out: Tensor, batch_size: int, grad_scale: float):
+        if not self.is_training:
+            raise log.TrainingModeRequired("output gradient")
+        if d_out.precision != self.precision:
+            raise log.UnsupportedTypeCast(d_out.precision, self.precision)
+        if d_out.cols() != self.linear_state.w.cols():
+            raise log.MismatchedDimensions("output gradient columns", self.linear_state.w.cols(), d_out.cols())
+        if d_out.rows() < batch_size:
+            raise log.MismatchedDimensions("output gradient rows vs explicit batch size", batch_size, d_out.rows())
+        if d_out.rows() > self.max_batch_size:
+            raise log.AllocationLimitExceeded(d_out.rows(), self.max_batch_size, "output gradient batches")
+        if not 0.0 < grad_scale < float("inf"):
+            raise log.InvalidConfiguration(f"Gradient scale {grad_scale} must be positive.")
+        self._check_mode(batch_size)
