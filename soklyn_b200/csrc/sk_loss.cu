@@ -61,11 +61,15 @@ int make_rows(sk_ctx *c, const sk_logits *x, bool need_gradient, loss::Rows *out
     return SK_OK;
 }
 
+#ifndef SK_NT
+#define SK_NT 256
+#endif
+constexpr int NT = SK_NT;
 template <typename T, class Op, bool ENT, bool GRAD>
 cudaError_t launch_rows(sk_ctx *c, const loss::Rows &r, const Op &op) {
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), loss::kThreads, 0, dim3(1), loss::row_kernel<T, Op, ENT, GRAD>, r, op);
+    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, 0, dim3(1), loss::row_kernel<T, NT, Op, ENT, GRAD>, r, op);
 }
 template <typename T, class Op> cudaError_t run_rows(sk_ctx *c, const loss::Rows &r, const Op &op, bool entropy) {
     if (r.d) return entropy ? launch_rows<T, Op, true, true>(c, r, op) : launch_rows<T, Op, false, true>(c, r, op);
@@ -87,14 +91,14 @@ template <typename T> cudaError_t sequence_impl(sk_ctx *c, const loss::Rows &r, 
 template <typename T> cudaError_t sequence_gradient_impl(sk_ctx *c, const loss::Rows &r, const int32_t *labels, const loss::Kept *kept) {
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), loss::kThreads, 0, dim3(1), loss::sequence_gradient_kernel<T>, r, labels, kept);
+    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, 0, dim3(1), loss::sequence_gradient_kernel<T, NT>, r, labels, kept);
 }
 template <typename T> cudaError_t distill_impl(sk_ctx *c, const loss::Rows &r, const loss::Distill &op) {
     static uint64_t attr_set[4] = {0, 0, 0, 0};   // devices 0..255
     const unsigned dev = (unsigned)c->device & 255u;
     constexpr size_t most = (loss::kMaxListClasses + 64) / 8;
     if (!(attr_set[dev >> 6] >> (dev & 63) & 1ull)) {
-        const cudaError_t e = cudaFuncSetAttribute(loss::distill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        const cudaError_t e = cudaFuncSetAttribute(loss::distill_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) return e;
         attr_set[dev >> 6] |= 1ull << (dev & 63);
     }
@@ -102,7 +106,7 @@ template <typename T> cudaError_t distill_impl(sk_ctx *c, const loss::Rows &r, c
     const size_t bytes = ((size_t)r.classes + 16 + 31) / 32 * 4;
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), loss::kThreads, bytes, dim3(1), loss::distill_kernel<T>, r, op);
+    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, bytes, dim3(1), loss::distill_kernel<T, NT>, r, op);
 }
 } // namespace
 

@@ -57,29 +57,119 @@ __device__ __forceinline__ double log_wide(float s) {
 constexpr double kEx2Low = 5.0e-8;
 __device__ __forceinline__ double log_sum(float s) { return log_wide(s) + kEx2Low * (1.0 - 1.0 / (double)s); }
 
-// ---- a row as aligned 16-byte units ---------------------------------------------------------
-// Rows of odd widths start anywhere: unit 0 begins at the 16-byte boundary at or below the first element, and the
-// elements of the first and last unit outside the row are never touched.
-template <typename T> struct Span {
-    static constexpr int V = 16 / sizeof(T);
-    const T *p;
-    uint32_t n, lead, units;
-    __device__ __forceinline__ Span(const T *first, uint32_t count) : p(first), n(count) {
-        lead = (uint32_t)(reinterpret_cast<uintptr_t>(first) % 16 / sizeof(T));
-        units = (lead + n + V - 1) / V;
+// ---- 16 bytes of a row, and pairs of f32 values ------------------------------------------------
+// Arithmetic is on pairs (add / mul / fma.rn.f32x2: two round-to-nearest operations in one instruction), because wide
+// rows of 16-bit logits are bound by instruction issue as much as by memory.
+using f32x2 = uint64_t;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f32x2 ex2_2(f32x2 t) { const float2 v = halves(t); return pair(ex2(v.x), ex2(v.y)); }
+// at least -200, where 2^t is 0 already: 0 * -inf does not arise
+__device__ __forceinline__ f32x2 floor2(f32x2 t) { const float2 v = halves(t); return pair(fmaxf(v.x, -200.0f), fmaxf(v.y, -200.0f)); }
+
+template <typename T> struct Unit;
+template <> struct Unit<float> {
+    static constexpr int V = 4;
+    uint4 q;
+    static constexpr uint32_t kNone = 0xFF800000u;        // -inf
+    __device__ __forceinline__ float max() const {
+        return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
     }
-    __device__ __forceinline__ int32_t start(uint32_t u) const { return (int32_t)(u * V) - (int32_t)lead; }
-    __device__ __forceinline__ bool whole(int32_t e0) const { return e0 >= 0 && (uint32_t)e0 + V <= n; }
-    __device__ __forceinline__ void load(uint32_t u, float (&v)[V]) const {
-        const int32_t e0 = start(u);
-        if (whole(e0)) {
-            unpack(load_pack<T, V>(p + e0), v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = e0 + j >= 0 && (uint32_t)(e0 + j) < n ? to_f32(p[e0 + j]) : -INFINITY;
-        }
+    __device__ __forceinline__ f32x2 get(int i) const {
+        return i ? pair(__uint_as_float(q.z), __uint_as_float(q.w)) : pair(__uint_as_float(q.x), __uint_as_float(q.y));
     }
+    __device__ __forceinline__ void set(int i, f32x2 v) {
+        const float2 f = halves(v);
+        if (i) { q.z = __float_as_uint(f.x); q.w = __float_as_uint(f.y); } else { q.x = __float_as_uint(f.x); q.y = __float_as_uint(f.y); }
+    }
+    __device__ __forceinline__ void put(int j, float v) { (&q.x)[j] = __float_as_uint(v); }
+    __device__ __forceinline__ float at(int j) const { return __uint_as_float((&q.x)[j]); }
+    __device__ __forceinline__ void drop(int j) { (&q.x)[j] = kNone; }
 };
+template <> struct Unit<__nv_bfloat16> {
+    static constexpr int V = 8;
+    uint4 q;
+    static constexpr uint32_t kNone = 0xFF80FF80u;
+    __device__ __forceinline__ float max() const {
+        auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
+        const __nv_bfloat162 m = __hmax2(__hmax2(h(q.x), h(q.y)), __hmax2(h(q.z), h(q.w)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    __device__ __forceinline__ f32x2 get(int i) const {
+        const uint32_t w = (&q.x)[i];
+        return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+    __device__ __forceinline__ void set(int i, f32x2 v) {
+        const float2 f = halves(v);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        (&q.x)[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    __device__ __forceinline__ float at(int j) const { const float2 f = halves(get(j / 2)); return j & 1 ? f.y : f.x; }
+    __device__ __forceinline__ void drop(int j) { uint32_t &w = (&q.x)[j / 2]; w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu); }
+};
+template <> struct Unit<__half> {
+    static constexpr int V = 8;
+    uint4 q;
+    static constexpr uint32_t kNone = 0xFC00FC00u;
+    __device__ __forceinline__ float max() const {
+        auto h = [](uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); };
+        const __half2 m = __hmax2(__hmax2(h(q.x), h(q.y)), __hmax2(h(q.z), h(q.w)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    __device__ __forceinline__ f32x2 get(int i) const {
+        const uint32_t w = (&q.x)[i];
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        return pair(f.x, f.y);
+    }
+    __device__ __forceinline__ void set(int i, f32x2 v) {
+        const float2 f = halves(v);
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        (&q.x)[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    __device__ __forceinline__ float at(int j) const { const float2 f = halves(get(j / 2)); return j & 1 ? f.y : f.x; }
+    __device__ __forceinline__ void drop(int j) { uint32_t &w = (&q.x)[j / 2]; w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu); }
+};
+template <typename T> __device__ __forceinline__ Unit<T> no_unit() {
+    constexpr uint32_t n = Unit<T>::kNone;
+    return Unit<T>{make_uint4(n, n, n, n)};
+}
+
+// ---- a row as aligned 16-byte units -------------------------------------------------------------
+// Rows of odd widths start anywhere: up to V - 1 elements before the first 16-byte boundary (head) and behind the last
+// one (tail) are taken one by one, each by one thread; nothing outside the row is touched.
+template <typename T> struct Span {
+    static constexpr int V = Unit<T>::V;
+    const T *p;
+    uint32_t n, head, units, tail;
+    __device__ __forceinline__ Span(const T *first, uint32_t count) : p(first), n(count) {
+        head = (uint32_t)((16 - reinterpret_cast<uintptr_t>(first) % 16) % 16 / sizeof(T));
+        head = head < n ? head : n;
+        units = (n - head) / V;
+        tail = n - head - units * V;
+    }
+    __device__ __forceinline__ Unit<T> load(uint32_t u) const { return Unit<T>{*reinterpret_cast<const uint4 *>(p + head + (size_t)u * V)}; }
+    __device__ __forceinline__ const T *tail_at() const { return p + (n - tail); }
+};
+// `count` < V elements from `p` on, -inf behind them.
+template <typename T> __device__ __forceinline__ Unit<T> part_unit(const T *p, uint32_t count) {
+    Unit<T> u = no_unit<T>();
+    T *e = reinterpret_cast<T *>(&u.q);
+#pragma unroll
+    for (int j = 0; j < Unit<T>::V - 1; ++j)
+        if ((uint32_t)j < count) e[j] = p[j];
+    return u;
+}
 
 // ---- row statistics ------------------------------------------------------------------------
 struct Stat { float m, s, u; };             // maximum, sum e, sum e t2 (t2 = t log2 e), relative to m
@@ -93,100 +183,150 @@ __device__ __forceinline__ void rescale(Stat &a, float to, float c) {
     a.m = to;
 }
 
-template <int V, bool ENT> __device__ __forceinline__ void accumulate(Stat &a, const float (&v)[V], float c_hi, float c_lo) {
-    float mx = v[0];
+template <typename T, int U, bool ENT> __device__ __forceinline__ void accumulate(Stat &a, const Unit<T> (&q)[U], float c_hi, float c_lo) {
+    float mx = q[0].max();
 #pragma unroll
-    for (int j = 1; j < V; ++j) mx = fmaxf(mx, v[j]);
+    for (int k = 1; k < U; ++k) mx = fmaxf(mx, q[k].max());
     if (mx > a.m) rescale(a, mx, c_hi);
     const float ref = a.m == -INFINITY ? 0.0f : a.m;
-    float s = 0.0f, u = 0.0f;
+    const f32x2 less = pair(-ref, -ref), hi = pair(c_hi, c_hi), lo = pair(c_lo, c_lo);
+    f32x2 s = 0, u = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float d = v[j] - ref, t = fmaf(d, c_hi, d * c_lo), e = ex2(t);
-        s += e;
-        if (ENT) u = fmaf(e, fmaxf(t, -200.0f), u);
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int i = 0; i < Unit<T>::V / 2; ++i) {
+            const f32x2 d = add2(q[k].get(i), less), t = fma2(d, hi, mul2(d, lo)), e = ex2_2(t);
+            s = add2(s, e);
+            if (ENT) u = fma2(e, floor2(t), u);
+        }
+    const float2 ss = halves(s);
+    a.s += ss.x + ss.y;
+    if (ENT) {
+        const float2 us = halves(u);
+        a.u += us.x + us.y;
     }
-    a.s += s;
-    if (ENT) a.u += u;
 }
 
-// One result from those of all threads of the block, in a fixed order. `red` alternates between rows (two of them), so
-// that one barrier is enough.
-template <bool ENT> __device__ __forceinline__ Stat merge(Stat a, Stat (&red)[kWarps], float c) {
-    const float m = warp_max(a.m);
-    rescale(a, m, c);
+// Units of one thread taken at once: their loads are in flight together.
+constexpr int kAhead = 4;
+
+// A thread's share of a row's statistics. `leave` takes (unit, first bit of the unit) and may drop classes from it.
+template <typename T, int NT, bool ENT, class Leave>
+__device__ __forceinline__ Stat scan_row(const Span<T> &sp, float c_hi, float c_lo, const Leave &leave) {
+    constexpr uint32_t V = Span<T>::V;
+    Stat a{-INFINITY, 0.0f, 0.0f};
+    for (uint32_t u = threadIdx.x; u < sp.units; u += NT * kAhead) {
+        Unit<T> q[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) q[k] = u + k * NT < sp.units ? sp.load(u + k * NT) : no_unit<T>();
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) leave(q[k], (u + k * NT + 1) * V, u + k * NT < sp.units);
+        accumulate<T, kAhead, ENT>(a, q, c_hi, c_lo);
+    }
+    if (threadIdx.x == 0 && sp.head) {
+        Unit<T> q[1] = {part_unit<T>(sp.p, sp.head)};
+        leave(q[0], V - sp.head, true);
+        accumulate<T, 1, ENT>(a, q, c_hi, c_lo);
+    }
+    if (threadIdx.x == NT - 1 && sp.tail) {
+        Unit<T> q[1] = {part_unit<T>(sp.tail_at(), sp.tail)};
+        leave(q[0], (sp.units + 1) * V, true);
+        accumulate<T, 1, ENT>(a, q, c_hi, c_lo);
+    }
+    return a;
+}
+struct LeaveNone {
+    template <typename U> __device__ __forceinline__ void operator()(U &, uint32_t, bool) const {}
+};
+
+// One result from those of all threads of the block, in a fixed order.
+template <int NT, bool ENT> __device__ __forceinline__ Stat merge(Stat a, Stat (&red)[NT / 32], float c) {
+    rescale(a, warp_max(a.m), c);
     a.s = warp_sum(a.s);
     if (ENT) a.u = warp_sum(a.u);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
     __syncthreads();
-    float all = red[0].m;
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) all = fmaxf(all, red[w].m);
-    Stat t{all, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        Stat b = red[w];
-        rescale(b, all, c);
-        t.s += b.s;
-        if (ENT) t.u += b.u;
-    }
-    return t;
+    Stat b{-INFINITY, 0.0f, 0.0f};
+    const uint32_t lane = threadIdx.x & 31;
+    if (lane < NT / 32) b = red[lane];
+    rescale(b, warp_max(b.m), c);
+    b.s = warp_sum(b.s);
+    if (ENT) b.u = warp_sum(b.u);
+    return b;
 }
 // A row all of whose classes are -inf has no distribution.
 __device__ __forceinline__ bool nothing(const Stat &a) { return a.m == -INFINITY && a.s == 0.0f; }
 
 // ---- gradient rows ---------------------------------------------------------------------------
 // Columns [from, cols) of row `row`: zero.
-template <typename T> __device__ __forceinline__ void zero_row(const Rows &r, uint32_t row, uint32_t from) {
-    if (!r.d) return;
+template <typename T, int NT> __device__ __forceinline__ void zero_row(const Rows &r, uint32_t row, uint32_t from) {
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols + from;
     const Span<T> sp(d, r.cols - from);
-    const T zero = from_f32<T>(0.0f);
-    Pack<T, Span<T>::V> z;
-#pragma unroll
-    for (int j = 0; j < Span<T>::V; ++j) z.v[j] = zero;
-    for (uint32_t u = threadIdx.x; u < sp.units; u += blockDim.x) {
-        const int32_t e0 = sp.start(u);
-        if (sp.whole(e0)) {
-            *reinterpret_cast<Pack<T, Span<T>::V> *>(d + e0) = z;
-        } else {
-            for (int j = 0; j < Span<T>::V; ++j)
-                if (e0 + j >= 0 && (uint32_t)(e0 + j) < sp.n) d[e0 + j] = zero;
-        }
-    }
+    for (uint32_t u = threadIdx.x; u < sp.units; u += NT) *reinterpret_cast<uint4 *>(d + sp.head + (size_t)u * Span<T>::V) = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < sp.head) d[threadIdx.x] = from_f32<T>(0.0f);
+    if (threadIdx.x < sp.tail) d[sp.n - sp.tail + threadIdx.x] = from_f32<T>(0.0f);
 }
 
 struct Coef { float a, b, at_label; };      // d_j = e_j (a + b t2_j), plus at_label at the label
 
+// One unit of the gradient; `at`: place of the label in it, or none.
+template <typename T, bool ENT> __device__ __forceinline__ void gradient_unit(Unit<T> &q, const Rows &r, float m, const Coef &k, uint32_t at) {
+    const f32x2 less = pair(-m, -m), hi = pair(r.c_hi, r.c_hi);
+#pragma unroll
+    for (int i = 0; i < Unit<T>::V / 2; ++i) {
+        const f32x2 d = add2(q.get(i), less), t = sizeof(T) == 4 ? fma2(d, hi, mul2(d, pair(r.c_lo, r.c_lo))) : mul2(d, hi), e = ex2_2(t);
+        f32x2 g = mul2(e, ENT ? fma2(floor2(t), pair(k.b, k.b), pair(k.a, k.a)) : pair(k.a, k.a));
+        if (at / 2 == (uint32_t)i) g = add2(g, at & 1 ? pair(0.0f, k.at_label) : pair(k.at_label, 0.0f));
+        q.set(i, g);
+    }
+}
+
 // The gradient of one row from its logits; `label` < 0: no correction. The gradient may lie where the logits lie: a
 // thread stores a unit after it has read it.
-template <typename T, bool ENT>
+template <typename T, int NT, bool ENT>
 __device__ __forceinline__ void write_row(const Rows &r, uint32_t row, float m, const Coef &k, int32_t label) {
-    constexpr int V = Span<T>::V;
+    constexpr uint32_t V = Span<T>::V;
     const size_t base = (size_t)row * r.cols;
     const T *x = reinterpret_cast<const T *>(r.x) + base;
     T *d = reinterpret_cast<T *>(r.d) + base;
     const Span<T> sp(x, r.classes);
-    const bool same = (reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) % 16 == 0;
-    for (uint32_t u = threadIdx.x; u < sp.units; u += blockDim.x) {
-        float v[V];
-        sp.load(u, v);
-        const int32_t e0 = sp.start(u);
+    const uint32_t rel = (uint32_t)(label - (int32_t)sp.head);         // huge for a label in the head, or none
+    if ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) % 16 == 0) {
+        for (uint32_t u = threadIdx.x; u < sp.units; u += NT * kAhead) {
+            Unit<T> q[kAhead];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float df = v[j] - m, t = sizeof(T) == 4 ? fmaf(df, r.c_hi, df * r.c_lo) : df * r.c_hi, e = ex2(t);
-            v[j] = ENT ? e * fmaf(k.b, fmaxf(t, -200.0f), k.a) : e * k.a;
-            if (label == e0 + j) v[j] += k.at_label;
+            for (int j = 0; j < kAhead; ++j)
+                if (u + j * NT < sp.units) q[j] = sp.load(u + j * NT);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (u + j * NT >= sp.units) break;
+                gradient_unit<T, ENT>(q[j], r, m, k, rel / V == u + j * NT ? rel % V : V);
+                *reinterpret_cast<uint4 *>(d + sp.head + (size_t)(u + j * NT) * V) = q[j].q;
+            }
         }
-        if (same && sp.whole(e0)) {
-            store_run<T, V>(d + e0, true, v);
-        } else {
+    } else {
+        for (uint32_t u = threadIdx.x; u < sp.units; u += NT) {
+            Unit<T> q = sp.load(u);
+            gradient_unit<T, ENT>(q, r, m, k, rel / V == u ? rel % V : V);
+            const T *e = reinterpret_cast<const T *>(&q.q);
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (e0 + j >= 0 && (uint32_t)(e0 + j) < sp.n) d[e0 + j] = from_f32<T>(v[j]);
+            for (int j = 0; j < (int)V; ++j) d[sp.head + (size_t)u * V + j] = e[j];
         }
     }
-    if (r.cols > r.classes) zero_row<T>(r, row, r.classes);
+    if ((threadIdx.x == 0 && sp.head) || (threadIdx.x == NT - 1 && sp.tail)) {
+        for (int side = 0; side < 2; ++side) {
+            if (threadIdx.x != (side ? NT - 1 : 0)) continue;
+            const uint32_t first = side ? sp.n - sp.tail : 0, count = side ? sp.tail : sp.head;
+            Unit<T> q = part_unit<T>(x + first, count);
+            const uint32_t in = (uint32_t)(label - (int32_t)first);
+            gradient_unit<T, ENT>(q, r, m, k, label >= 0 && in < count ? in : V);
+            const T *e = reinterpret_cast<const T *>(&q.q);
+#pragma unroll
+            for (int j = 0; j < (int)V - 1; ++j)
+                if ((uint32_t)j < count) d[first + j] = e[j];
+        }
+    }
+    if (r.cols > r.classes) zero_row<T, NT>(r, row, r.classes);
 }
 
 // ---- losses on the log-probability of one class per row ------------------------------------------
@@ -309,9 +449,9 @@ struct SequenceLogprob {
 };
 
 // One block per row.
-template <typename T, class Op, bool ENT, bool GRAD>
-__global__ void __launch_bounds__(kThreads) row_kernel(Rows r, Op op) {
-    __shared__ Stat red[kWarps];
+template <typename T, int NT, class Op, bool ENT, bool GRAD>
+__global__ void __launch_bounds__(NT) row_kernel(Rows r, Op op) {
+    __shared__ Stat red[NT / 32];
     const uint32_t row = blockIdx.x;
     const bool first = threadIdx.x == 0;
     grid_ready();
@@ -321,21 +461,15 @@ __global__ void __launch_bounds__(kThreads) row_kernel(Rows r, Op op) {
     float at = 0.0f;
     if (label >= 0) {
         at = to_f32(x[label]);
-        const Span<T> sp(x, r.classes);
-        for (uint32_t u = threadIdx.x; u < sp.units; u += kThreads) {
-            float v[Span<T>::V];
-            sp.load(u, v);
-            accumulate<Span<T>::V, ENT>(a, v, r.c_hi, r.c_lo);
-        }
-        a = merge<ENT>(a, red, r.c_hi);
+        a = merge<NT, ENT>(scan_row<T, NT, ENT>(Span<T>(x, r.classes), r.c_hi, r.c_lo, LeaveNone()), red, r.c_hi);
     }
     if (label < 0 || nothing(a)) {
         if (first) op.skip(row);
-        if (GRAD) zero_row<T>(r, row, 0);
+        if (GRAD) zero_row<T, NT>(r, row, 0);
         return;
     }
     const Coef k = op.finish(r, row, a, at, first);
-    if (GRAD) write_row<T, ENT>(r, row, a.m, k, label);
+    if (GRAD) write_row<T, NT, ENT>(r, row, a.m, k, label);
 }
 
 // ---- preference loss: sequences ---------------------------------------------------------------------
@@ -418,16 +552,16 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(Pairs p) {
 }
 
 // d = k g (1[j = l] - p_j) from the kept maximum and sum. A row without a sum got no log-probability.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sequence_gradient_kernel(Rows r, const int32_t *labels, const Kept *kept) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) sequence_gradient_kernel(Rows r, const int32_t *labels, const Kept *kept) {
     const uint32_t row = blockIdx.x;
     grid_ready();
     const Kept k = kept[row];
     if (k.s == 0.0f || k.g == 0.0f) {
-        zero_row<T>(r, row, 0);
+        zero_row<T, NT>(r, row, 0);
         return;
     }
-    write_row<T, false>(r, row, k.m, Coef{-r.k * k.g / k.s, 0.0f, r.k * k.g}, labels[row]);
+    write_row<T, NT, false>(r, row, k.m, Coef{-r.k * k.g / k.s, 0.0f, r.k * k.g}, labels[row]);
 }
 
 // ---- distillation --------------------------------------------------------------------------------
@@ -452,11 +586,11 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
 //                         [ (Q + r) p_j - q_j                          at its classes   ]
 // S is a sum of its own over the classes outside: 1 - sum p_k would cancel. A bit per class in shared memory says which
 // those are; it also finds indices given twice, whose masses add at their class.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(Rows r, Distill t) {
-    constexpr int V = Span<T>::V;
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_kernel(Rows r, Distill t) {
+    constexpr uint32_t V = Span<T>::V;
     extern __shared__ uint32_t bits[];
-    __shared__ Stat red[kWarps];
+    __shared__ Stat red[NT / 32];
     __shared__ int32_t idx[kMaxList];
     __shared__ float val[kMaxList], sx[kMaxList];
     const uint32_t row = blockIdx.x, lane = threadIdx.x & 31;
@@ -464,24 +598,24 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(Rows r, Distill t) {
     grid_ready();
     const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
     const Span<T> sp(x, r.classes);
-    const uint32_t words = (sp.units * V + 31) / 32;
+    const uint32_t words = ((sp.units + 1) * V + sp.tail + 31) / 32;   // unit u has bits from (u + 1) V on, the head those below V
     const float w = t.weights ? t.weights[row] : 1.0f;
     auto nothing_to_learn = [&] {
         if (first) t.loss[row] = 0.0f;
-        if (r.d) zero_row<T>(r, row, 0);
+        if (r.d) zero_row<T, NT>(r, row, 0);
     };
     if (w == 0.0f) return nothing_to_learn();
-    for (uint32_t i = threadIdx.x; i < words; i += kThreads) bits[i] = 0;
+    for (uint32_t i = threadIdx.x; i < words; i += NT) bits[i] = 0;
     __syncthreads();
     bool twice = false;
-    for (uint32_t i = threadIdx.x; i < t.k; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < t.k; i += NT) {
         int32_t c = t.indices[(size_t)row * t.k + i];
         if (c >= 0 && (uint32_t)c >= r.classes) { atomicOr(r.err, kErrList); c = -1; }
         idx[i] = c;
         val[i] = c >= 0 ? teacher_value(t, (size_t)row * t.k + i) : -INFINITY;
         sx[i] = c >= 0 ? to_f32(x[c]) : -INFINITY;
         if (c >= 0) {
-            const uint32_t b = (uint32_t)c + sp.lead;
+            const uint32_t b = (uint32_t)c + V - sp.head;
             twice |= (atomicOr(&bits[b / 32], 1u << (b % 32)) >> (b % 32)) & 1u;
         }
     }
@@ -492,17 +626,13 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(Rows r, Distill t) {
                 if (idx[o] == idx[i]) return false;
         return idx[i] >= 0;
     };
-    Stat a{-INFINITY, 0.0f, 0.0f};
-    for (uint32_t u = threadIdx.x; u < sp.units; u += kThreads) {
-        float v[V];
-        sp.load(u, v);
-        const uint32_t mark = bits[u * V / 32] >> (u * V % 32) & ((1u << V) - 1u);
+    const Stat outside_list = scan_row<T, NT, false>(sp, r.c_hi, r.c_lo, [&](Unit<T> &q, uint32_t bit, bool there) {
+        const uint32_t mark = there ? bits[bit / 32] >> (bit % 32) & ((1u << V) - 1u) : 0;
         if (mark)
 #pragma unroll
-            for (int j = 0; j < V; ++j) if (mark >> j & 1u) v[j] = -INFINITY;
-        accumulate<V, false>(a, v, r.c_hi, r.c_lo);
-    }
-    a = merge<false>(a, red, r.c_hi);
+            for (int j = 0; j < (int)V; ++j) if (mark >> j & 1u) q.drop(j);
+    });
+    Stat a = merge<NT, false>(outside_list, red, r.c_hi);
     // the list: every warp goes through it for itself
     float top = -INFINITY, best = -INFINITY;
     for (uint32_t i = lane; i < t.k; i += 32) { top = fmaxf(top, val[i]); best = fmaxf(best, sx[i]); }
@@ -545,10 +675,10 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(Rows r, Distill t) {
     // k = loss scale / T, the gradient's factor w T loss scale = w k T^2
     const float f = (float)((double)w * (double)r.k * t.factor);
     const float outside = a.s > 0.0f ? (float)((double)total / (double)s - rest / (double)a.s) : 0.0f;
-    write_row<T, false>(r, row, m, Coef{f * outside, 0.0f, 0.0f}, -1);
+    write_row<T, NT, false>(r, row, m, Coef{f * outside, 0.0f, 0.0f}, -1);
     __syncthreads();                        // the list's classes are written again, with their own values
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
-    for (uint32_t i = threadIdx.x; i < t.k; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < t.k; i += NT) {
         if (!leads(i)) continue;
         float q = 0.0f;
         for (uint32_t o = i; o < (twice ? t.k : i + 1); ++o)
