@@ -1107,6 +1107,7 @@ int sk_step_begin(sk_ctx *c, uint32_t slot) {
         if ((rc = check_cuda(c, cudaStreamBeginCapture(c->record_stream, cudaStreamCaptureModeThreadLocal), "begin stream capture"))) return rc;
         c->user_stream = c->stream;
         c->stream = c->record_stream;
+        launch_shape = 0;
     }
     c->step_open = (int)slot;
     c->step_capturing = record;
@@ -1143,9 +1144,9 @@ int sk_step_end(sk_ctx *c) {
     if (rc) { if (graph) cudaGraphDestroy(graph); cudaGetLastError(); return rc; }
     if (g.exec) {
         cudaGraphExecUpdateResultInfo info;
-        if (cudaGraphExecUpdate(g.exec, graph, &info) == cudaSuccess) {
+        if (g.shape == launch_shape && cudaGraphExecUpdate(g.exec, graph, &info) == cudaSuccess) {
             c->step_stats[1]++;
-        } else {   // another sequence of kernels than the slot's last step
+        } else {   // another sequence of kernels, or of cluster dimensions, than the slot's last step
             cudaGetLastError();
             cudaGraphExecDestroy(g.exec);
             g.exec = nullptr;
@@ -1155,6 +1156,7 @@ int sk_step_end(sk_ctx *c) {
         rc = check_cuda(c, cudaGraphInstantiate(&g.exec, graph, 0), "instantiate step graph");
         if (rc) { g.exec = nullptr; cudaGraphDestroy(graph); return rc; }
         c->step_stats[0]++;
+        g.shape = launch_shape;
     }
     cudaGraphDestroy(graph);
     rc = check_cuda(c, cudaGraphLaunch(g.exec, c->stream), "launch step graph");

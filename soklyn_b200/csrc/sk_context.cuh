@@ -53,7 +53,7 @@ struct sk_ctx {
     const void *fused_colsum_key = nullptr;   // d_prenorm of the layer whose partial sums sit in the workspace
     uint32_t fused_colsum_groups = 0, fused_colsum_batch = 0;
     // whole-step graphs (sk_step_begin / sk_step_end)
-    struct StepGraph { cudaGraphExec_t exec = nullptr; bool warmed = false; };
+    struct StepGraph { cudaGraphExec_t exec = nullptr; bool warmed = false; uint64_t shape = 0; };   // shape: launch_shape of the record
     StepGraph step_graphs[SK_STEP_SLOTS];
     int step_open = -1;                    // slot between begin and end
     bool step_capturing = false;

@@ -33,6 +33,10 @@ __device__ __forceinline__ void grid_ready() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// What the launches of this thread asked for beside their arguments: an executable graph that is updated in place keeps
+// the cluster dimensions of its nodes (cudaGraphExecUpdate takes over new arguments, grids and functions), so a record
+// whose launches differ in them from the last one has to be instantiated anew.
+inline thread_local uint64_t launch_shape = 0;
 template <class... P, class... A>
 inline cudaError_t launch_step(cudaStream_t stream, bool overlap, dim3 grid, uint32_t threads, size_t smem, dim3 cluster, void (*kernel)(P...), A &&...args) {
     cudaLaunchConfig_t cfg{};
@@ -52,6 +56,7 @@ inline cudaError_t launch_step(cudaStream_t stream, bool overlap, dim3 grid, uin
         attr[cfg.numAttrs++].val.clusterDim.z = cluster.z;
     }
     cfg.attrs = attr;
+    launch_shape = (launch_shape ^ (((uint64_t)cluster.x << 42) + ((uint64_t)cluster.y << 21) + ((uint64_t)cluster.z << 1) + overlap)) * 1099511628211ull + 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
     if (e != cudaSuccess) cudaGetLastError();   // reported here: not again by the next call that asks for the last error
     return e;
