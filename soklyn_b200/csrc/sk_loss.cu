@@ -61,52 +61,64 @@ int make_rows(sk_ctx *c, const sk_logits *x, bool need_gradient, loss::Rows *out
     return SK_OK;
 }
 
-#ifndef SK_NT
-#define SK_NT 256
+// Threads of a block and blocks of a cluster for a row; the reasons stand beside Team. `twice`: the row is read again.
+constexpr size_t kWarpRow = 32 * loss::kWarpUnits * 16, kPerThread = 256;
+#ifndef SK_MAXT
+#define SK_MAXT 256
 #endif
-constexpr int NT = SK_NT;
-template <typename T, class Op, bool ENT, bool GRAD>
-cudaError_t launch_rows(sk_ctx *c, const loss::Rows &r, const Op &op) {
+constexpr uint32_t kMostThreads = SK_MAXT;
+struct RowPlan { uint32_t threads, ranks; };
+RowPlan plan_row(const sk_ctx *c, const loss::Rows &r, size_t one, bool twice) {
+    const size_t bytes = (size_t)r.classes * one, sms = (size_t)c->num_sms;
+    if (bytes <= kWarpRow) return RowPlan{32, 1};
+    RowPlan plan{64, 1};
+    while (plan.threads < kMostThreads && bytes > plan.threads * kPerThread) plan.threads *= 2;
+    while (twice && plan.ranks < loss::kMaxCluster && bytes > plan.ranks * plan.threads * kPerThread) plan.ranks *= 2;
+    // few rows: more threads for each, then more blocks, down to 32 bytes per thread
+    while (plan.threads < kMostThreads && r.rows * plan.threads < sms * 1024 && bytes >= plan.threads * 64) plan.threads *= 2;
+    while (plan.ranks < loss::kMaxCluster && r.rows * plan.ranks * 2 <= sms && bytes >= plan.ranks * plan.threads * 64) plan.ranks *= 2;
+    return plan;
+}
+template <typename T, class Op, int SUMS, bool GRAD> cudaError_t launch_rows(sk_ctx *c, const loss::Rows &r, const Op &op) {
+    constexpr int warp_sums = SUMS ? loss::kMasked : loss::kSums;
+    const RowPlan plan = plan_row(c, r, sizeof(T), GRAD);
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, 0, dim3(1), loss::row_kernel<T, NT, Op, ENT, GRAD>, r, op);
-}
-template <typename T, class Op> cudaError_t run_rows(sk_ctx *c, const loss::Rows &r, const Op &op, bool entropy) {
-    if (r.d) return entropy ? launch_rows<T, Op, true, true>(c, r, op) : launch_rows<T, Op, false, true>(c, r, op);
-    return entropy ? launch_rows<T, Op, true, false>(c, r, op) : launch_rows<T, Op, false, false>(c, r, op);
+    if (plan.threads == 32)
+        return launch_step(c->stream, overlaps(c), dim3((r.rows + loss::kWarps - 1) / loss::kWarps), loss::kThreads, 0, dim3(1), loss::warp_kernel<T, Op, warp_sums, GRAD>, r, op);
+    auto kernel = plan.threads == 64 ? loss::row_kernel<T, 64, Op, SUMS, GRAD> : plan.threads == 128 ? loss::row_kernel<T, 128, Op, SUMS, GRAD> : loss::row_kernel<T, kMostThreads, Op, SUMS, GRAD>;
+    return launch_step(c->stream, overlaps(c), dim3(r.rows * plan.ranks), plan.threads, 0, dim3(plan.ranks), kernel, r, op);
 }
 
 template <typename T> cudaError_t label_impl(sk_ctx *c, const loss::Rows &r, const loss::LabelLogprob &op) {
-    return op.entropy ? launch_rows<T, loss::LabelLogprob, true, false>(c, r, op) : launch_rows<T, loss::LabelLogprob, false, false>(c, r, op);
+    return op.entropy ? launch_rows<T, loss::LabelLogprob, loss::kEntropy, false>(c, r, op) : launch_rows<T, loss::LabelLogprob, loss::kSums, false>(c, r, op);
 }
 template <typename T> cudaError_t label_backward_impl(sk_ctx *c, const loss::Rows &r, const loss::LabelLogprobBackward &op) {
-    return op.d_entropy ? launch_rows<T, loss::LabelLogprobBackward, true, true>(c, r, op) : launch_rows<T, loss::LabelLogprobBackward, false, true>(c, r, op);
+    return op.d_entropy ? launch_rows<T, loss::LabelLogprobBackward, loss::kEntropy, true>(c, r, op) : launch_rows<T, loss::LabelLogprobBackward, loss::kSums, true>(c, r, op);
 }
 template <typename T> cudaError_t policy_impl(sk_ctx *c, const loss::Rows &r, const loss::Policy &op) {
-    return run_rows<T>(c, r, op, op.entropy || op.eta != 0.0f);
+    if (op.entropy || op.eta != 0.0f) return r.d ? launch_rows<T, loss::Policy, loss::kEntropy, true>(c, r, op) : launch_rows<T, loss::Policy, loss::kEntropy, false>(c, r, op);
+    return r.d ? launch_rows<T, loss::Policy, loss::kSums, true>(c, r, op) : launch_rows<T, loss::Policy, loss::kSums, false>(c, r, op);
 }
 template <typename T> cudaError_t sequence_impl(sk_ctx *c, const loss::Rows &r, const loss::SequenceLogprob &op) {
-    return launch_rows<T, loss::SequenceLogprob, false, false>(c, r, op);
+    return launch_rows<T, loss::SequenceLogprob, loss::kSums, false>(c, r, op);
 }
 template <typename T> cudaError_t sequence_gradient_impl(sk_ctx *c, const loss::Rows &r, const int32_t *labels, const loss::Kept *kept) {
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, 0, dim3(1), loss::sequence_gradient_kernel<T, NT>, r, labels, kept);
+    const size_t bytes = (size_t)r.classes * sizeof(T);
+    auto kernel = bytes <= 64 * kPerThread ? loss::sequence_gradient_kernel<T, 64> : bytes <= 128 * kPerThread ? loss::sequence_gradient_kernel<T, 128> : loss::sequence_gradient_kernel<T, 256>;
+    const uint32_t threads = bytes <= 64 * kPerThread ? 64 : bytes <= 128 * kPerThread ? 128 : 256;
+    return launch_step(c->stream, overlaps(c), dim3(r.rows), threads, 0, dim3(1), kernel, r, labels, kept);
 }
 template <typename T> cudaError_t distill_impl(sk_ctx *c, const loss::Rows &r, const loss::Distill &op) {
-    static uint64_t attr_set[4] = {0, 0, 0, 0};   // devices 0..255
-    const unsigned dev = (unsigned)c->device & 255u;
-    constexpr size_t most = (loss::kMaxListClasses + 64) / 8;
-    if (!(attr_set[dev >> 6] >> (dev & 63) & 1ull)) {
-        const cudaError_t e = cudaFuncSetAttribute(loss::distill_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
-        if (e != cudaSuccess) return e;
-        attr_set[dev >> 6] |= 1ull << (dev & 63);
-    }
-    // a bit for every element of the row's units: up to two units more than its classes fill
-    const size_t bytes = ((size_t)r.classes + 16 + 31) / 32 * 4;
+    const RowPlan plan = plan_row(c, r, sizeof(T), r.d != nullptr);
+    const size_t units = (size_t)r.classes * sizeof(T) / 16, bytes = ((units + plan.ranks - 1) / plan.ranks + 2) * (16 / sizeof(T)) / 8 + 4;   // a bit per class of a part, its edges in units of their own
+    const uint32_t threads = std::max(plan.threads, 64u);
+    auto kernel = threads == 64 ? loss::distill_kernel<T, 64> : threads == 128 ? loss::distill_kernel<T, 128> : loss::distill_kernel<T, kMostThreads>;
     c->launches++;
     c->loss_launches++;
-    return launch_step(c->stream, overlaps(c), dim3(r.rows), NT, bytes, dim3(1), loss::distill_kernel<T, NT>, r, op);
+    return launch_step(c->stream, overlaps(c), dim3(r.rows * plan.ranks), threads, bytes, dim3(plan.ranks), kernel, r, op);
 }
 } // namespace
 

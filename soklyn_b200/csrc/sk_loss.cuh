@@ -12,11 +12,12 @@
 
 #include "sk_device.cuh"
 #include "sk_epilogue.cuh"
+#include "sk_tc_ptx.cuh"
 
 namespace sk {
 namespace loss {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;      // of the pair kernel
 constexpr uint32_t kMaxList = 512;          // entries of a teacher's list
 constexpr uint32_t kMaxListClasses = 1u << 20;   // a bit for each class fits shared memory
 constexpr float kLn2 = 0.693147180559945f;
@@ -55,7 +56,14 @@ __device__ __forceinline__ double log_wide(float s) {
 // the sum over a sequence would not average out. It made 8e-6 of a preference margin of sequences that differ by
 // hundreds of rows.
 constexpr double kEx2Low = 5.0e-8;
-__device__ __forceinline__ double log_sum(float s) { return log_wide(s) + kEx2Low * (1.0 - 1.0 / (double)s); }
+__device__ __forceinline__ double log_sum(float s) { return log_wide(s) + (double)((float)kEx2Low * (1.0f - __fdividef(1.0f, s))); }
+
+// The largest of a warp's values, in every lane; one instruction on sm_100a. NaN only if all are.
+__device__ __forceinline__ float max_of_warp(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 
 // ---- 16 bytes of a row, and pairs of f32 values ------------------------------------------------
 // Arithmetic is on pairs (add / mul / fma.rn.f32x2: two round-to-nearest operations in one instruction), because wide
@@ -75,8 +83,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ f32x2 ex2_2(f32x2 t) { const float2 v = halves(t); return pair(ex2(v.x), ex2(v.y)); }
-// at least -200, where 2^t is 0 already: 0 * -inf does not arise
-__device__ __forceinline__ f32x2 floor2(f32x2 t) { const float2 v = halves(t); return pair(fmaxf(v.x, -200.0f), fmaxf(v.y, -200.0f)); }
 
 template <typename T> struct Unit;
 template <> struct Unit<float> {
@@ -93,8 +99,6 @@ template <> struct Unit<float> {
         const float2 f = halves(v);
         if (i) { q.z = __float_as_uint(f.x); q.w = __float_as_uint(f.y); } else { q.x = __float_as_uint(f.x); q.y = __float_as_uint(f.y); }
     }
-    __device__ __forceinline__ void put(int j, float v) { (&q.x)[j] = __float_as_uint(v); }
-    __device__ __forceinline__ float at(int j) const { return __uint_as_float((&q.x)[j]); }
     __device__ __forceinline__ void drop(int j) { (&q.x)[j] = kNone; }
 };
 template <> struct Unit<__nv_bfloat16> {
@@ -115,8 +119,10 @@ template <> struct Unit<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
         (&q.x)[i] = *reinterpret_cast<const uint32_t *>(&h);
     }
-    __device__ __forceinline__ float at(int j) const { const float2 f = halves(get(j / 2)); return j & 1 ? f.y : f.x; }
-    __device__ __forceinline__ void drop(int j) { uint32_t &w = (&q.x)[j / 2]; w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu); }
+    __device__ __forceinline__ void drop(int j) {
+        uint32_t &w = (&q.x)[j / 2];
+        w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu);
+    }
 };
 template <> struct Unit<__half> {
     static constexpr int V = 8;
@@ -137,8 +143,10 @@ template <> struct Unit<__half> {
         const __half2 h = __floats2half2_rn(f.x, f.y);
         (&q.x)[i] = *reinterpret_cast<const uint32_t *>(&h);
     }
-    __device__ __forceinline__ float at(int j) const { const float2 f = halves(get(j / 2)); return j & 1 ? f.y : f.x; }
-    __device__ __forceinline__ void drop(int j) { uint32_t &w = (&q.x)[j / 2]; w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu); }
+    __device__ __forceinline__ void drop(int j) {
+        uint32_t &w = (&q.x)[j / 2];
+        w = j & 1 ? (w & 0xFFFFu) | (kNone & 0xFFFF0000u) : (w & 0xFFFF0000u) | (kNone & 0xFFFFu);
+    }
 };
 template <typename T> __device__ __forceinline__ Unit<T> no_unit() {
     constexpr uint32_t n = Unit<T>::kNone;
@@ -174,20 +182,27 @@ template <typename T> __device__ __forceinline__ Unit<T> part_unit(const T *p, u
 // ---- row statistics ------------------------------------------------------------------------
 struct Stat { float m, s, u; };             // maximum, sum e, sum e t2 (t2 = t log2 e), relative to m
 
-// (s, u) of a partial sum relative to m, seen from the larger maximum `to`.
-__device__ __forceinline__ void rescale(Stat &a, float to, float c) {
+// What is summed beside e. kSums: nothing; the exponent is the product with both parts of log2(e) / T. kEntropy: e t2 as
+// well, from which the second part's effect on s follows at once (with_low), so that one product is enough. A class at
+// -inf makes NaN of e t2 = 0 * -inf; such a row is taken again with kMasked, which bounds t2 at -200, where e is 0 already.
+enum Sums : int { kSums = 0, kEntropy = 1, kMasked = 2 };
+// (s, u) of a partial sum relative to m, seen from the larger maximum `to`. An exponent beyond f32 makes NaN of u as one
+// class's does, unless that is bounded.
+template <int SUMS> __device__ __forceinline__ void rescale(Stat &a, float to, float c) {
     if (a.m == -INFINITY) { a.m = to; return; }   // holds no class (or only NaN, which s keeps)
     const float d = (a.m - to) * c, f = ex2(d);
-    a.u = f * (a.u + fmaxf(d, -200.0f) * a.s);
+    if (SUMS) a.u = f * fmaf(SUMS == kMasked ? fmaxf(d, -200.0f) : d, a.s, a.u);
     a.s *= f;
     a.m = to;
 }
 
-template <typename T, int U, bool ENT> __device__ __forceinline__ void accumulate(Stat &a, const Unit<T> (&q)[U], float c_hi, float c_lo) {
+__device__ __forceinline__ f32x2 floor2(f32x2 t) { const float2 v = halves(t); return pair(fmaxf(v.x, -200.0f), fmaxf(v.y, -200.0f)); }
+
+template <typename T, int U, int SUMS> __device__ __forceinline__ void accumulate(Stat &a, const Unit<T> (&q)[U], float c_hi, float c_lo) {
     float mx = q[0].max();
 #pragma unroll
     for (int k = 1; k < U; ++k) mx = fmaxf(mx, q[k].max());
-    if (mx > a.m) rescale(a, mx, c_hi);
+    if (mx > a.m) rescale<SUMS>(a, mx, c_hi);
     const float ref = a.m == -INFINITY ? 0.0f : a.m;
     const f32x2 less = pair(-ref, -ref), hi = pair(c_hi, c_hi), lo = pair(c_lo, c_lo);
     f32x2 s = 0, u = 0;
@@ -195,144 +210,233 @@ template <typename T, int U, bool ENT> __device__ __forceinline__ void accumulat
     for (int k = 0; k < U; ++k)
 #pragma unroll
         for (int i = 0; i < Unit<T>::V / 2; ++i) {
-            const f32x2 d = add2(q[k].get(i), less), t = fma2(d, hi, mul2(d, lo)), e = ex2_2(t);
+            const f32x2 d = add2(q[k].get(i), less), t = SUMS == kSums ? fma2(d, hi, mul2(d, lo)) : mul2(d, hi), e = ex2_2(t);
             s = add2(s, e);
-            if (ENT) u = fma2(e, floor2(t), u);
+            if (SUMS) u = fma2(e, SUMS == kMasked ? floor2(t) : t, u);
         }
     const float2 ss = halves(s);
     a.s += ss.x + ss.y;
-    if (ENT) {
+    if (SUMS) {
         const float2 us = halves(u);
         a.u += us.x + us.y;
     }
 }
+// sum 2^(d (c_hi + c_lo)) = sum e (1 + ln2 d c_lo) up to 1e-12
+__device__ __forceinline__ void with_low(Stat &a, float c_hi, float c_lo) { a.s = fmaf(kLn2 * c_lo / c_hi, a.u, a.s); }
+__device__ __forceinline__ bool masked(const Stat &a) { return a.u != a.u && a.s == a.s; }
 
-// Units of one thread taken at once: their loads are in flight together.
-constexpr int kAhead = 4;
-
-// A thread's share of a row's statistics. `leave` takes (unit, first bit of the unit) and may drop classes from it.
-template <typename T, int NT, bool ENT, class Leave>
-__device__ __forceinline__ Stat scan_row(const Span<T> &sp, float c_hi, float c_lo, const Leave &leave) {
-    constexpr uint32_t V = Span<T>::V;
-    Stat a{-INFINITY, 0.0f, 0.0f};
-    for (uint32_t u = threadIdx.x; u < sp.units; u += NT * kAhead) {
-        Unit<T> q[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) q[k] = u + k * NT < sp.units ? sp.load(u + k * NT) : no_unit<T>();
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) leave(q[k], (u + k * NT + 1) * V, u + k * NT < sp.units);
-        accumulate<T, kAhead, ENT>(a, q, c_hi, c_lo);
-    }
-    if (threadIdx.x == 0 && sp.head) {
-        Unit<T> q[1] = {part_unit<T>(sp.p, sp.head)};
-        leave(q[0], V - sp.head, true);
-        accumulate<T, 1, ENT>(a, q, c_hi, c_lo);
-    }
-    if (threadIdx.x == NT - 1 && sp.tail) {
-        Unit<T> q[1] = {part_unit<T>(sp.tail_at(), sp.tail)};
-        leave(q[0], (sp.units + 1) * V, true);
-        accumulate<T, 1, ENT>(a, q, c_hi, c_lo);
-    }
-    return a;
-}
-struct LeaveNone {
-    template <typename U> __device__ __forceinline__ void operator()(U &, uint32_t, bool) const {}
-};
-
-// One result from those of all threads of the block, in a fixed order.
-template <int NT, bool ENT> __device__ __forceinline__ Stat merge(Stat a, Stat (&red)[NT / 32], float c) {
-    rescale(a, warp_max(a.m), c);
-    a.s = warp_sum(a.s);
-    if (ENT) a.u = warp_sum(a.u);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    Stat b{-INFINITY, 0.0f, 0.0f};
-    const uint32_t lane = threadIdx.x & 31;
-    if (lane < NT / 32) b = red[lane];
-    rescale(b, warp_max(b.m), c);
-    b.s = warp_sum(b.s);
-    if (ENT) b.u = warp_sum(b.u);
-    return b;
-}
 // A row all of whose classes are -inf has no distribution.
 __device__ __forceinline__ bool nothing(const Stat &a) { return a.m == -INFINITY && a.s == 0.0f; }
 
-// ---- gradient rows ---------------------------------------------------------------------------
-// Columns [from, cols) of row `row`: zero.
-template <typename T, int NT> __device__ __forceinline__ void zero_row(const Rows &r, uint32_t row, uint32_t from) {
-    T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols + from;
-    const Span<T> sp(d, r.cols - from);
-    for (uint32_t u = threadIdx.x; u < sp.units; u += NT) *reinterpret_cast<uint4 *>(d + sp.head + (size_t)u * Span<T>::V) = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x < sp.head) d[threadIdx.x] = from_f32<T>(0.0f);
-    if (threadIdx.x < sp.tail) d[sp.n - sp.tail + threadIdx.x] = from_f32<T>(0.0f);
-}
+// ---- who works on a row -----------------------------------------------------------------------------
+// A row of up to 4 KB is held by one warp in registers. Wider ones belong to a block, which reads them again for the
+// gradient, from the L2 cache: at 256 bytes of a row per thread the rows in flight fit it and there are still enough warps.
+// Measured with gradients (log-probability, 1 GiB read and written, 164 us of memory): 16384 bf16 columns 185 us with 128
+// threads, 231 with 256; 32768 columns 241, 190, 234 with 128, 256, 512. Above 64 KB a cluster shares the row: 131072
+// columns 215 us on four blocks, 246 on one, whose rows in flight leave the cache. Without a gradient nothing is read
+// again and one block is faster (131072 columns 90 us against 111).
+// Tried and slower: rows kept in shared memory, copied ahead of time by a warp of its own (32768 columns 216 us and
+// more): one block per SM has too few warps to hide its reductions and exponentials.
+constexpr int kAhead = 4;                   // units of a thread whose loads are in flight together
+constexpr uint32_t kMaxCluster = 8;
+constexpr int kWarpUnits = 8;               // units of a lane of a row held by a warp
+struct alignas(16) Message { float m, s, u; int flag; };
+
+// A block's part of a row: units [first, first + units) of its span, with the head before unit 0 and the tail behind the last.
+template <typename T> struct Part {
+    static constexpr int V = Unit<T>::V;
+    uint32_t begin, head, units, tail;      // begin: element of the row at which the units start
+    __device__ __forceinline__ Part(const Span<T> &sp, uint32_t rank, uint32_t ranks) {
+        const uint32_t u0 = (uint32_t)((uint64_t)sp.units * rank / ranks), u1 = (uint32_t)((uint64_t)sp.units * (rank + 1) / ranks);
+        begin = sp.head + u0 * V;
+        units = u1 - u0;
+        head = rank == 0 ? sp.head : 0;
+        tail = rank == ranks - 1 ? sp.tail : 0;
+    }
+    __device__ __forceinline__ Unit<T> load(const T *x, uint32_t u) const { return Unit<T>{*reinterpret_cast<const uint4 *>(x + begin + (size_t)u * V)}; }
+    __device__ __forceinline__ bool holds(uint32_t j) const { return j + head >= begin && j < begin + units * V + tail; }
+    // place of element j among bits or units: the head's unit, the units, the tail's unit; elements count from the head's end
+    __device__ __forceinline__ uint32_t place(uint32_t j) const { return j - begin + V; }
+};
 
 struct Coef { float a, b, at_label; };      // d_j = e_j (a + b t2_j), plus at_label at the label
 
-// One unit of the gradient; `at`: place of the label in it, or none.
-template <typename T, bool ENT> __device__ __forceinline__ void gradient_unit(Unit<T> &q, const Rows &r, float m, const Coef &k, uint32_t at) {
-    const f32x2 less = pair(-m, -m), hi = pair(r.c_hi, r.c_hi);
+// NT threads that work on one row together.
+template <int NT> struct Team {
+    struct Shared { Stat red[2][NT / 32]; Message box[2][kMaxCluster]; Coef coef; };
+    Shared &sh;
+    uint32_t tid, lane, rank, ranks, merged, met;
+    __device__ __forceinline__ explicit Team(Shared &s) : sh(s), tid(threadIdx.x), lane(threadIdx.x & 31), rank(tc::cluster_rank()), ranks(tc::cluster_size()), merged(0), met(0) {
+        if (ranks > 1) cluster_arrive();
+    }
+    // Every team that was set up either meets or leaves.
+    __device__ __forceinline__ void leave() { if (ranks > 1 && met == 0) cluster_wait(); }
+    static __device__ __forceinline__ void cluster_arrive() {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    static __device__ __forceinline__ void cluster_wait() {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // The block's statistics from those of its threads, in every thread, in a fixed order.
+    template <int SUMS> __device__ __forceinline__ Stat merge(Stat a, float c) {
+        Stat(&red)[NT / 32] = sh.red[merged++ & 1];      // the other one may still be read
+        rescale<SUMS>(a, max_of_warp(a.m), c);
+        a.s = warp_sum(a.s);
+        if (SUMS) a.u = warp_sum(a.u);
+        if (lane == 0) red[tid / 32] = a;
+        __syncthreads();
+        Stat b[NT / 32], t{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) { b[w] = red[w]; t.m = fmaxf(t.m, b[w].m); }
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) {
+            rescale<SUMS>(b[w], t.m, c);
+            t.s += b[w].s;
+            if (SUMS) t.u += b[w].u;
+        }
+        return t;
+    }
+    // The cluster's from those of its blocks, in rank order. All blocks of the cluster, the same number of times.
+    template <int SUMS> __device__ __forceinline__ Stat meet(const Stat &a, int flag, float c, int *any) {
+        if (ranks == 1) { *any = flag; return a; }
+        if (met == 0) cluster_wait();                    // every block runs: its shared memory may be written
+        Message(&box)[kMaxCluster] = sh.box[met++ & 1];  // of the other one a block may still be reading
+        if (tid < ranks) {
+            const uint32_t at = tc::map_shared(tc::smem_u32(&box[rank]), tid);
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.s)), "r"(__float_as_uint(a.u)), "r"(flag) : "memory");
+        }
+        tc::cluster_sync();
+        Stat t{-INFINITY, 0.0f, 0.0f};
+        *any = 0;
+        for (uint32_t i = 0; i < ranks; ++i) t.m = fmaxf(t.m, box[i].m);
+        for (uint32_t i = 0; i < ranks; ++i) {
+            Stat b{box[i].m, box[i].s, box[i].u};
+            rescale<SUMS>(b, t.m, c);
+            t.s += b.s;
+            if (SUMS) t.u += b.u;
+            *any |= box[i].flag;
+        }
+        return t;
+    }
+    // A thread's share of the statistics of this block's part of the row at x. Units that do not fill a group are summed one
+    // by one, the head and the tail by the form that takes places that are no classes. `leave` takes (unit, its place).
+    template <typename T, int SUMS, class Leave>
+    __device__ __forceinline__ Stat scan(const T *x, const Part<T> &p, float c_hi, float c_lo, const Leave &leave) const {
+        constexpr uint32_t V = Part<T>::V;
+        Stat a{-INFINITY, 0.0f, 0.0f};
+        for (uint32_t u = tid; u < p.units; u += NT * kAhead) {
+            Unit<T> q[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (u + k * NT < p.units) q[k] = p.load(x, u + k * NT);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (u + k * NT < p.units) leave(q[k], (u + k * NT + 1) * V);
+            if (u + (kAhead - 1) * NT < p.units) {
+                accumulate<T, kAhead, SUMS>(a, q, c_hi, c_lo);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kAhead - 1; ++k)
+                    if (u + k * NT < p.units) accumulate<T, 1, SUMS>(a, reinterpret_cast<const Unit<T>(&)[1]>(q[k]), c_hi, c_lo);
+            }
+        }
+        constexpr int kEdge = SUMS ? kMasked : kSums;
+        if (tid == 0 && p.head) {
+            Unit<T> q[1] = {part_unit<T>(x, p.head)};
+            leave(q[0], V - p.head);
+            accumulate<T, 1, kEdge>(a, q, c_hi, c_lo);
+        }
+        if (tid == NT - 1 && p.tail) {
+            Unit<T> q[1] = {part_unit<T>(x + p.begin + p.units * V, p.tail)};
+            leave(q[0], (p.units + 1) * V);
+            accumulate<T, 1, kEdge>(a, q, c_hi, c_lo);
+        }
+        return a;
+    }
+};
+struct LeaveNone {
+    template <typename U> __device__ __forceinline__ void operator()(U &, uint32_t) const {}
+};
+
+// ---- gradient rows ---------------------------------------------------------------------------
+// Columns [from, to) of row `row`: zero.
+template <typename T, int NT> __device__ __forceinline__ void zero_row(const Rows &r, uint32_t row, uint32_t from, uint32_t to, uint32_t tid) {
+    if (from >= to) return;
+    T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols + from;
+    const Span<T> sp(d, to - from);
+    for (uint32_t u = tid; u < sp.units; u += NT) *reinterpret_cast<uint4 *>(d + sp.head + (size_t)u * Span<T>::V) = make_uint4(0, 0, 0, 0);
+    if (tid < sp.head) d[tid] = from_f32<T>(0.0f);
+    if (tid < sp.tail) d[sp.n - sp.tail + tid] = from_f32<T>(0.0f);
+}
+
+template <typename T, int SUMS> __device__ __forceinline__ float gradient_of(float x, const Rows &r, float m, const Coef &k) {
+    const float d = x - m, t = sizeof(T) == 4 ? fmaf(d, r.c_hi, d * r.c_lo) : d * r.c_hi;   // 16 bits hide the second part
+    return ex2(t) * (SUMS ? fmaf(k.b, SUMS == kMasked ? fmaxf(t, -200.0f) : t, k.a) : k.a);
+}
+template <typename T, int SUMS> __device__ __forceinline__ void gradient_unit(Unit<T> &q, const Rows &r, float m, const Coef &k) {
 #pragma unroll
     for (int i = 0; i < Unit<T>::V / 2; ++i) {
-        const f32x2 d = add2(q.get(i), less), t = sizeof(T) == 4 ? fma2(d, hi, mul2(d, pair(r.c_lo, r.c_lo))) : mul2(d, hi), e = ex2_2(t);
-        f32x2 g = mul2(e, ENT ? fma2(floor2(t), pair(k.b, k.b), pair(k.a, k.a)) : pair(k.a, k.a));
-        if (at / 2 == (uint32_t)i) g = add2(g, at & 1 ? pair(0.0f, k.at_label) : pair(k.at_label, 0.0f));
-        q.set(i, g);
+        const float2 x = halves(q.get(i));
+        q.set(i, pair(gradient_of<T, SUMS>(x.x, r, m, k), gradient_of<T, SUMS>(x.y, r, m, k)));
     }
 }
 
-// The gradient of one row from its logits; `label` < 0: no correction. The gradient may lie where the logits lie: a
-// thread stores a unit after it has read it.
-template <typename T, int NT, bool ENT>
-__device__ __forceinline__ void write_row(const Rows &r, uint32_t row, float m, const Coef &k, int32_t label) {
-    constexpr uint32_t V = Span<T>::V;
+// Up to V - 1 elements of a row at its head or tail.
+template <typename T, int SUMS>
+__device__ __forceinline__ void write_edge(const Rows &r, T *d, Unit<T> q, uint32_t first, uint32_t count, float m, const Coef &k, int32_t label, T at_label) {
+    gradient_unit<T, SUMS ? kMasked : kSums>(q, r, m, k);
+    const T *e = reinterpret_cast<const T *>(&q.q);
+#pragma unroll
+    for (uint32_t j = 0; j < Unit<T>::V - 1; ++j)
+        if (j < count) d[first + j] = e[j];
+    if (label >= 0 && (uint32_t)label - first < count) d[label] = at_label;
+}
+// One unit at element `at` of the row; the label's element is written behind its unit by the thread that wrote that.
+template <typename T> __device__ __forceinline__ void write_unit(T *d, const Unit<T> &q, size_t at, bool whole, bool has_label, int32_t label, T at_label) {
+    if (whole) {
+        *reinterpret_cast<uint4 *>(d + at) = q.q;
+    } else {                                // the gradient lies on another offset within 16 bytes than the logits
+        const T *e = reinterpret_cast<const T *>(&q.q);
+#pragma unroll
+        for (int j = 0; j < Unit<T>::V; ++j) d[at + j] = e[j];
+    }
+    if (has_label) d[label] = at_label;
+}
+// The gradient of this block's part of a row from its logits; label < 0: none. It may lie where the logits lie: a thread
+// stores a unit after it has read it.
+template <typename T, int NT, int SUMS>
+__device__ __forceinline__ void write_row(const Rows &r, uint32_t row, const Part<T> &p, uint32_t rank, uint32_t ranks, float m, const Coef &k, int32_t label, float at) {
+    constexpr uint32_t V = Part<T>::V;
     const size_t base = (size_t)row * r.cols;
     const T *x = reinterpret_cast<const T *>(r.x) + base;
     T *d = reinterpret_cast<T *>(r.d) + base;
-    const Span<T> sp(x, r.classes);
-    const uint32_t rel = (uint32_t)(label - (int32_t)sp.head);         // huge for a label in the head, or none
-    if ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) % 16 == 0) {
-        for (uint32_t u = threadIdx.x; u < sp.units; u += NT * kAhead) {
-            Unit<T> q[kAhead];
+    const bool whole = reinterpret_cast<uintptr_t>(d + p.begin) % 16 == 0;
+    const uint32_t label_unit = (uint32_t)(label - (int32_t)p.begin) / V;      // beyond all units if it is not here
+    const T at_label = from_f32<T>(gradient_of<T, SUMS ? kMasked : kSums>(at, r, m, k) + k.at_label);
+    for (uint32_t u = threadIdx.x; u < p.units; u += NT * kAhead) {
+        Unit<T> q[kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (u + j * NT < sp.units) q[j] = sp.load(u + j * NT);
+        for (int j = 0; j < kAhead; ++j)
+            if (u + j * NT < p.units) q[j] = p.load(x, u + j * NT);
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                if (u + j * NT >= sp.units) break;
-                gradient_unit<T, ENT>(q[j], r, m, k, rel / V == u + j * NT ? rel % V : V);
-                *reinterpret_cast<uint4 *>(d + sp.head + (size_t)(u + j * NT) * V) = q[j].q;
-            }
-        }
-    } else {
-        for (uint32_t u = threadIdx.x; u < sp.units; u += NT) {
-            Unit<T> q = sp.load(u);
-            gradient_unit<T, ENT>(q, r, m, k, rel / V == u ? rel % V : V);
-            const T *e = reinterpret_cast<const T *>(&q.q);
-#pragma unroll
-            for (int j = 0; j < (int)V; ++j) d[sp.head + (size_t)u * V + j] = e[j];
+        for (int j = 0; j < kAhead; ++j) {
+            if (u + j * NT >= p.units) break;
+            gradient_unit<T, SUMS>(q[j], r, m, k);
+            write_unit<T>(d, q[j], p.begin + (size_t)(u + j * NT) * V, whole, label_unit == u + j * NT, label, at_label);
         }
     }
-    if ((threadIdx.x == 0 && sp.head) || (threadIdx.x == NT - 1 && sp.tail)) {
-        for (int side = 0; side < 2; ++side) {
-            if (threadIdx.x != (side ? NT - 1 : 0)) continue;
-            const uint32_t first = side ? sp.n - sp.tail : 0, count = side ? sp.tail : sp.head;
-            Unit<T> q = part_unit<T>(x + first, count);
-            const uint32_t in = (uint32_t)(label - (int32_t)first);
-            gradient_unit<T, ENT>(q, r, m, k, label >= 0 && in < count ? in : V);
-            const T *e = reinterpret_cast<const T *>(&q.q);
-#pragma unroll
-            for (int j = 0; j < (int)V - 1; ++j)
-                if ((uint32_t)j < count) d[first + j] = e[j];
-        }
-    }
-    if (r.cols > r.classes) zero_row<T, NT>(r, row, r.classes);
+    if (threadIdx.x == 0 && p.head) write_edge<T, SUMS>(r, d, part_unit<T>(x, p.head), 0, p.head, m, k, label, at_label);
+    if (threadIdx.x == NT - 1 && p.tail)
+        write_edge<T, SUMS>(r, d, part_unit<T>(x + p.begin + p.units * V, p.tail), p.begin + p.units * V, p.tail, m, k, label, at_label);
+    if (rank == ranks - 1) zero_row<T, NT>(r, row, r.classes, r.cols, threadIdx.x);
 }
 
 // ---- losses on the log-probability of one class per row ------------------------------------------
-// Each says which rows count and which class they ask for (begin), and turns a row's statistics into outputs and the
-// coefficients of its gradient (finish; called by every thread with the same values, `first` is one of them).
-struct RowIn { float x; int32_t label; };
+// Each fetches what a row brings along (fetch), says which class it asks for (label_of; below 0: the row does not count),
+// and turns its statistics into outputs and the coefficients of its gradient (finish; called by a warp with the same
+// values, `first` is one of its threads).
 __device__ __forceinline__ int32_t checked_label(const Rows &r, int32_t label, bool first) {
     if (label >= 0 && (uint32_t)label >= r.classes) {
         if (first) atomicOr(r.err, kErrLabel);
@@ -346,12 +450,14 @@ __device__ __forceinline__ double log_prob(const Rows &r, const Stat &a, double 
 struct LabelLogprob {
     const int32_t *labels;
     float *logp, *entropy;
-    __device__ __forceinline__ int32_t begin(const Rows &r, uint32_t row, bool first) const { return checked_label(r, labels[row], first); }
+    struct In { int32_t label; };
+    __device__ __forceinline__ In fetch(uint32_t row) const { return In{labels[row]}; }
+    static __device__ __forceinline__ int32_t label_of(const In &in) { return in.label; }
     __device__ __forceinline__ void skip(uint32_t row) const {
         logp[row] = 0.0f;
         if (entropy) entropy[row] = 0.0f;
     }
-    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, bool first) const {
+    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &, bool first) const {
         if (first) {
             const double log_s = log_sum(a.s);
             logp[row] = (float)log_prob(r, a, log_s, x);
@@ -365,11 +471,13 @@ struct LabelLogprob {
 struct LabelLogprobBackward {
     const int32_t *labels;
     const float *d_logp, *d_entropy;
-    __device__ __forceinline__ int32_t begin(const Rows &r, uint32_t row, bool first) const { return checked_label(r, labels[row], first); }
+    struct In { int32_t label; float g, h; };
+    __device__ __forceinline__ In fetch(uint32_t row) const { return In{labels[row], d_logp[row], d_entropy ? d_entropy[row] * kLn2 : 0.0f}; }
+    static __device__ __forceinline__ int32_t label_of(const In &in) { return in.label; }
     __device__ __forceinline__ void skip(uint32_t) const {}
-    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float, bool) const {
-        const float g = d_logp[row], h = d_entropy ? d_entropy[row] * kLn2 : 0.0f, f = r.k / a.s;
-        return Coef{f * (h * (a.u / a.s) - g), -f * h, r.k * g};
+    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t, const Stat &a, float, const In &in, bool) const {
+        const float f = r.k / a.s;
+        return Coef{f * (in.h * (a.u / a.s) - in.g), -f * in.h, r.k * in.g};
     }
 };
 
@@ -379,9 +487,11 @@ struct Policy {
     const float *old, *advantages, *ref, *weights;
     float lo, hi, beta, eta;
     float *loss, *logp, *kl, *entropy;
-    __device__ __forceinline__ int32_t begin(const Rows &r, uint32_t row, bool first) const {
-        return weights && weights[row] == 0.0f ? -1 : checked_label(r, actions[row], first);
+    struct In { int32_t label; float w, old, adv, ref; };
+    __device__ __forceinline__ In fetch(uint32_t row) const {
+        return In{actions[row], weights ? weights[row] : 1.0f, old[row], advantages[row], ref ? ref[row] : 0.0f};
     }
+    static __device__ __forceinline__ int32_t label_of(const In &in) { return in.w == 0.0f ? -1 : in.label; }
     __device__ __forceinline__ void skip(uint32_t row) const {
         loss[row] = logp[row] = kl[row] = 0.0f;
         if (entropy) entropy[row] = 0.0f;
@@ -394,11 +504,11 @@ struct Policy {
         p = fmaf(p, d, 1.0f / 24.0f); p = fmaf(p, d, 1.0f / 6.0f); p = fmaf(p, d, 0.5f);
         return p * d * d;
     }
-    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, bool first) const {
+    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &in, bool first) const {
         const double log_s = log_sum(a.s), lp = log_prob(r, a, log_s, x);
-        const float w = weights ? weights[row] : 1.0f, adv = advantages[row];
-        const float rho = expf((float)(lp - (double)old[row]));
-        const float d = ref ? (float)((double)ref[row] - lp) : 0.0f, h = (float)(log_s - (double)(a.u / a.s * kLn2));
+        const float w = in.w, adv = in.adv;
+        const float rho = expf((float)(lp - (double)in.old));
+        const float d = ref ? (float)((double)in.ref - lp) : 0.0f, h = (float)(log_s - (double)(a.u / a.s * kLn2));
         const float plain = rho * adv, held = fminf(fmaxf(rho, lo), hi) * adv;
         const bool clipped = (adv > 0.0f && rho > hi) || (adv < 0.0f && rho < lo);
         float g = clipped ? 0.0f : -plain;
@@ -428,15 +538,17 @@ struct SequenceLogprob {
     uint32_t sequences;
     float *row_logp;
     Kept *kept;
-    __device__ __forceinline__ int32_t begin(const Rows &r, uint32_t row, bool first) const {
+    struct In { int32_t label; };
+    __device__ __forceinline__ In fetch(uint32_t row) const {
         const bool inside = (int64_t)offsets[0] <= (int64_t)row && (int64_t)row < (int64_t)offsets[sequences];
-        return inside ? checked_label(r, labels[row], first) : -1;
+        return In{inside ? labels[row] : -1};
     }
+    static __device__ __forceinline__ int32_t label_of(const In &in) { return in.label; }
     __device__ __forceinline__ void skip(uint32_t row) const {
         row_logp[row] = 0.0f;
         kept[row] = Kept{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, bool first) const {
+    __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &, bool first) const {
         if (first) {
             const double lp = log_prob(r, a, log_sum(a.s), x);
             row_logp[row] = (float)lp;
@@ -448,28 +560,100 @@ struct SequenceLogprob {
     }
 };
 
-// One block per row.
-template <typename T, int NT, class Op, bool ENT, bool GRAD>
+// A cluster (mostly of one block) per row.
+template <typename T, int NT, class Op, int SUMS, bool GRAD>
 __global__ void __launch_bounds__(NT) row_kernel(Rows r, Op op) {
-    __shared__ Stat red[NT / 32];
-    const uint32_t row = blockIdx.x;
-    const bool first = threadIdx.x == 0;
+    __shared__ typename Team<NT>::Shared shared;
+    Team<NT> team(shared);
+    const uint32_t row = blockIdx.x / team.ranks;
+    const bool first = team.tid == 0 && team.rank == 0;
     grid_ready();
     const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
-    const int32_t label = op.begin(r, row, first);
-    Stat a{-INFINITY, 0.0f, 0.0f};
+    const typename Op::In in = op.fetch(row);
+    const int32_t label = checked_label(r, Op::label_of(in), first);
+    auto skip = [&] {
+        team.leave();
+        if (first) op.skip(row);
+        if (GRAD) zero_row<T, NT>(r, row, (uint32_t)((uint64_t)r.cols * team.rank / team.ranks), (uint32_t)((uint64_t)r.cols * (team.rank + 1) / team.ranks), team.tid);
+    };
+    if (label < 0) return skip();
+    const float at = to_f32(x[label]);
+    const Part<T> part(Span<T>(x, r.classes), team.rank, team.ranks);
+    int any;
+    Stat a = team.template merge<SUMS>(team.template scan<T, SUMS>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi);
+    a = team.template meet<SUMS>(a, 0, r.c_hi, &any);
+    bool again = false;
+    if (SUMS == kEntropy && masked(a)) {
+        again = true;
+        a = team.template merge<kMasked>(team.template scan<T, kMasked>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi);
+        a = team.template meet<kMasked>(a, 0, r.c_hi, &any);
+    }
+    if (SUMS) with_low(a, r.c_hi, r.c_lo);
+    if (nothing(a)) return skip();
+    // a few hundred instructions: one warp's
+    if (team.tid < 32) {
+        const Coef k = op.finish(r, row, a, at, in, first);
+        if (GRAD && team.tid == 0) shared.coef = k;
+    }
+    if (!GRAD) return;
+    __syncthreads();
+    const Coef k = shared.coef;
+    if (SUMS == kEntropy && again) write_row<T, NT, kMasked>(r, row, part, team.rank, team.ranks, a.m, k, label, at);
+    else write_row<T, NT, SUMS>(r, row, part, team.rank, team.ranks, a.m, k, label, at);
+}
+
+// A warp per row, which it holds in registers: up to 32 x kWarpUnits units and the edges. SUMS: kSums or kMasked.
+template <typename T, class Op, int SUMS, bool GRAD>
+__global__ void __launch_bounds__(kThreads) warp_kernel(Rows r, Op op) {
+    constexpr uint32_t V = Part<T>::V;
+    const uint32_t lane = threadIdx.x & 31, row = blockIdx.x * kWarps + threadIdx.x / 32;
+    const bool first = lane == 0;
+    grid_ready();
+    if (row >= r.rows) return;
+    const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
+    const typename Op::In in = op.fetch(row);
+    const Part<T> p(Span<T>(x, r.classes), 0, 1);
+    Unit<T> q[kWarpUnits], edge = no_unit<T>();
+#pragma unroll
+    for (int k = 0; k < kWarpUnits; ++k) q[k] = lane + k * 32 < p.units ? p.load(x, lane + k * 32) : no_unit<T>();
+    const uint32_t side = lane == 0 ? p.head : lane == 31 ? p.tail : 0, from = lane == 0 ? 0 : p.begin + p.units * V;
+    if (side) edge = part_unit<T>(x + from, side);
+    const int32_t label = checked_label(r, Op::label_of(in), first);
     float at = 0.0f;
+    Stat a{-INFINITY, 0.0f, 0.0f};
     if (label >= 0) {
         at = to_f32(x[label]);
-        a = merge<NT, ENT>(scan_row<T, NT, ENT>(Span<T>(x, r.classes), r.c_hi, r.c_lo, LeaveNone()), red, r.c_hi);
+#pragma unroll
+        for (int k = 0; k < kWarpUnits; k += 2)
+            if (k * 32 < p.units) accumulate<T, 2, SUMS>(a, reinterpret_cast<const Unit<T>(&)[2]>(q[k]), r.c_hi, r.c_lo);
+        if (side) accumulate<T, 1, SUMS>(a, reinterpret_cast<const Unit<T>(&)[1]>(edge), r.c_hi, r.c_lo);
+        rescale<SUMS>(a, max_of_warp(a.m), r.c_hi);
+        a.s = warp_sum(a.s);
+        if (SUMS) {
+            a.u = warp_sum(a.u);
+            with_low(a, r.c_hi, r.c_lo);
+        }
     }
+    T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
     if (label < 0 || nothing(a)) {
         if (first) op.skip(row);
-        if (GRAD) zero_row<T, NT>(r, row, 0);
+        if (GRAD) zero_row<T, 32>(r, row, 0, r.cols, lane);
         return;
     }
-    const Coef k = op.finish(r, row, a, at, first);
-    if (GRAD) write_row<T, NT, ENT>(r, row, a.m, k, label);
+    const Coef k = op.finish(r, row, a, at, in, first);
+    if (!GRAD) return;
+    const bool whole = reinterpret_cast<uintptr_t>(d + p.begin) % 16 == 0;
+    const uint32_t label_unit = (uint32_t)(label - (int32_t)p.begin) / V;
+    const T at_label = from_f32<T>(gradient_of<T, SUMS>(at, r, a.m, k) + k.at_label);
+#pragma unroll
+    for (int j = 0; j < kWarpUnits; ++j) {
+        const uint32_t u = lane + j * 32;
+        if (u >= p.units) break;
+        gradient_unit<T, SUMS>(q[j], r, a.m, k);
+        write_unit<T>(d, q[j], p.begin + (size_t)u * V, whole, label_unit == u, label, at_label);
+    }
+    if (side) write_edge<T, SUMS>(r, d, edge, from, side, a.m, k, label, at_label);
+    zero_row<T, 32>(r, row, r.classes, r.cols, lane);
 }
 
 // ---- preference loss: sequences ---------------------------------------------------------------------
@@ -558,10 +742,12 @@ __global__ void __launch_bounds__(NT) sequence_gradient_kernel(Rows r, const int
     grid_ready();
     const Kept k = kept[row];
     if (k.s == 0.0f || k.g == 0.0f) {
-        zero_row<T, NT>(r, row, 0);
+        zero_row<T, NT>(r, row, 0, r.cols, threadIdx.x);
         return;
     }
-    write_row<T, NT, false>(r, row, k.m, Coef{-r.k * k.g / k.s, 0.0f, r.k * k.g}, labels[row]);
+    const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
+    const int32_t label = labels[row];
+    write_row<T, NT, kSums>(r, row, Part<T>(Span<T>(x, r.classes), 0, 1), 0, 1, k.m, Coef{-r.k * k.g / k.s, 0.0f, r.k * k.g}, label, to_f32(x[label]));
 }
 
 // ---- distillation --------------------------------------------------------------------------------
@@ -579,112 +765,135 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
                                      : to_f32(reinterpret_cast<const __nv_bfloat16 *>(d.values)[i]);
 }
 
-// One block per row. With q_k the teacher's probabilities of its list (a softmax over it, or exp(v_k / T - lse)), Q
-// their sum, r = 1 - Q the mass outside (given lse; else 0) and S the student's probability outside the list,
+// With q_k the teacher's probabilities of its list (a softmax over it, or exp(v_k / T - lse)), Q their sum, r = 1 - Q the
+// mass outside (given lse; else 0) and S the student's probability outside the list,
 //   loss = w T^2 [ sum q_k (log q_k - log p_k) + r (log r - log S) ]
 //   d_j  = w T loss_scale [ (Q + r) p_j - r e_j / (sum of e outside)   outside the list ]
 //                         [ (Q + r) p_j - q_j                          at its classes   ]
-// S is a sum of its own over the classes outside: 1 - sum p_k would cancel. A bit per class in shared memory says which
-// those are; it also finds indices given twice, whose masses add at their class.
+// S is a sum of its own over the classes outside (1 - sum p_k would cancel): a bit for each class of the block's part says
+// which are listed, and these count as -inf where the row is summed; they are written by themselves behind the rest of the
+// gradient. Setting its bit also tells an entry whether its class was given before; the masses then add at the class.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_kernel(Rows r, Distill t) {
-    constexpr uint32_t V = Span<T>::V;
+    constexpr uint32_t V = Unit<T>::V;
     extern __shared__ uint32_t bits[];
-    __shared__ Stat red[NT / 32];
+    __shared__ typename Team<NT>::Shared shared;
     __shared__ int32_t idx[kMaxList];
-    __shared__ float val[kMaxList], sx[kMaxList];
-    const uint32_t row = blockIdx.x, lane = threadIdx.x & 31;
-    const bool first = threadIdx.x == 0;
+    __shared__ struct { float m, to_mass, f, total, of_s, outside; bool dead; } found;   // what the list's warp made of it
+    __shared__ float val[kMaxList], sx[kMaxList], share[kMaxList];      // the teacher's logit, the student's, the teacher's share (not normalised)
+    Team<NT> team(shared);
+    const uint32_t row = blockIdx.x / team.ranks, tid = team.tid, lane = team.lane;
+    const bool first = tid == 0 && team.rank == 0;
     grid_ready();
     const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
-    const Span<T> sp(x, r.classes);
-    const uint32_t words = ((sp.units + 1) * V + sp.tail + 31) / 32;   // unit u has bits from (u + 1) V on, the head those below V
     const float w = t.weights ? t.weights[row] : 1.0f;
     auto nothing_to_learn = [&] {
+        team.leave();
         if (first) t.loss[row] = 0.0f;
-        if (r.d) zero_row<T, NT>(r, row, 0);
+        if (r.d) zero_row<T, NT>(r, row, (uint32_t)((uint64_t)r.cols * team.rank / team.ranks), (uint32_t)((uint64_t)r.cols * (team.rank + 1) / team.ranks), tid);
     };
     if (w == 0.0f) return nothing_to_learn();
-    for (uint32_t i = threadIdx.x; i < words; i += NT) bits[i] = 0;
-    __syncthreads();
-    bool twice = false;
-    for (uint32_t i = threadIdx.x; i < t.k; i += NT) {
+    const Part<T> part(Span<T>(x, r.classes), team.rank, team.ranks);
+    const uint32_t words = ((part.units + 2) * V + 31) / 32;
+    for (uint32_t i = tid; i < words; i += NT) bits[i] = 0;
+    for (uint32_t i = tid; i < t.k; i += NT) {
         int32_t c = t.indices[(size_t)row * t.k + i];
-        if (c >= 0 && (uint32_t)c >= r.classes) { atomicOr(r.err, kErrList); c = -1; }
+        if (c >= 0 && (uint32_t)c >= r.classes) { if (team.rank == 0) atomicOr(r.err, kErrList); c = -1; }
         idx[i] = c;
         val[i] = c >= 0 ? teacher_value(t, (size_t)row * t.k + i) : -INFINITY;
         sx[i] = c >= 0 ? to_f32(x[c]) : -INFINITY;
-        if (c >= 0) {
-            const uint32_t b = (uint32_t)c + V - sp.head;
+    }
+    __syncthreads();
+    auto mine = [&](uint32_t i) { return idx[i] >= 0 && part.holds((uint32_t)idx[i]); };
+    float top = -INFINITY;
+    bool some = false;
+    for (uint32_t i = lane; i < t.k; i += 32) { top = fmaxf(top, val[i]); some |= idx[i] >= 0; }
+    top = max_of_warp(top);
+    some = __any_sync(0xffffffffu, some);
+    const double shift = t.lse ? (double)t.lse[row] : (double)top * r.inv_t;
+    bool twice = false;
+    for (uint32_t i = tid; i < t.k; i += NT) {
+        if (mine(i)) {
+            const uint32_t b = part.place((uint32_t)idx[i]);
             twice |= (atomicOr(&bits[b / 32], 1u << (b % 32)) >> (b % 32)) & 1u;
         }
+        share[i] = val[i] == -INFINITY ? 0.0f : expf((float)((double)val[i] * r.inv_t - shift));
     }
     twice = __syncthreads_or(twice);
+    Stat a = team.template merge<kSums>(team.template scan<T, kSums>(x, part, r.c_hi, r.c_lo, [&](Unit<T> &q, uint32_t place) {
+        const uint32_t mark = bits[place / 32] >> (place % 32) & ((1u << V) - 1u);
+        if (mark)
+#pragma unroll
+            for (int j = 0; j < (int)V; ++j) if (mark >> j & 1u) q.drop(j);
+    }), r.c_hi);
+    int any;
+    a = team.template meet<kSums>(a, twice, r.c_hi, &any);
+    twice = any;
     auto leads = [&](uint32_t i) {          // the first entry of its class
         if (twice)
             for (uint32_t o = 0; o < i; ++o)
                 if (idx[o] == idx[i]) return false;
         return idx[i] >= 0;
     };
-    const Stat outside_list = scan_row<T, NT, false>(sp, r.c_hi, r.c_lo, [&](Unit<T> &q, uint32_t bit, bool there) {
-        const uint32_t mark = there ? bits[bit / 32] >> (bit % 32) & ((1u << V) - 1u) : 0;
-        if (mark)
-#pragma unroll
-            for (int j = 0; j < (int)V; ++j) if (mark >> j & 1u) q.drop(j);
-    });
-    Stat a = merge<NT, false>(outside_list, red, r.c_hi);
-    // the list: every warp goes through it for itself
-    float top = -INFINITY, best = -INFINITY;
-    for (uint32_t i = lane; i < t.k; i += 32) { top = fmaxf(top, val[i]); best = fmaxf(best, sx[i]); }
-    top = warp_max(top);
-    best = warp_max(best);
-    const bool lost = __any_sync(0xffffffffu, [&] { bool n = false; for (uint32_t i = lane; i < t.k; i += 32) n |= idx[i] >= 0; return n; }());
-    const float m = fmaxf(a.m, best);
-    if ((!t.lse && (!lost || top == -INFINITY)) || (m == -INFINITY && a.s == 0.0f)) return nothing_to_learn();
-    rescale(a, m, r.c_hi);
-    const double shift = t.lse ? (double)t.lse[row] : (double)top * r.inv_t;
-    auto raw_q = [&](uint32_t i) { return val[i] == -INFINITY ? 0.0f : expf((float)((double)val[i] * r.inv_t - shift)); };
-    float listed = 0.0f;
-    double mass = 0.0;
-    for (uint32_t i = lane; i < t.k; i += 32) {
-        const float d = sx[i] - m, e = ex2(fmaf(d, r.c_hi, d * r.c_lo));
-        if (leads(i)) listed += e;
-        mass += (double)raw_q(i);
-    }
-    listed = warp_sum(listed);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-    const float s = a.s + listed, to_mass = t.lse ? 1.0f : (float)(1.0 / mass);
-    double rest = t.lse ? 1.0 - mass : 0.0;
-    if (rest <= kLeastTail) rest = 0.0;
-    const float total = t.lse ? (float)(mass + rest) : 1.0f;
-    if (threadIdx.x < 32) {
-        const double log_s = log_sum(s), log_mass = t.lse ? 0.0 : log_wide((float)mass);
-        double l = 0.0;
+    if (tid < 32) {                         // the list is one warp's
+        float best = -INFINITY, listed = 0.0f;
+        for (uint32_t i = lane; i < t.k; i += 32) best = fmaxf(best, sx[i]);
+        const float m = fmaxf(a.m, max_of_warp(best));
+        const bool dead = (!t.lse && (!some || top == -INFINITY)) || (m == -INFINITY && a.s == 0.0f);
+        rescale<kSums>(a, m, r.c_hi);
+        double mass = 0.0;
         for (uint32_t i = lane; i < t.k; i += 32) {
-            const double log_q = (double)val[i] * r.inv_t - shift - log_mass;
-            const float q = raw_q(i) * to_mass;
-            if (q != 0.0f) l += (double)q * (log_q - (((double)sx[i] - (double)m) * r.inv_t - log_s));
+            const float d = sx[i] - m, e = ex2(fmaf(d, r.c_hi, d * r.c_lo));
+            if (leads(i)) listed += e;
+            mass += (double)share[i];
         }
+        listed = warp_sum(listed);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (rest > 0.0) l += rest * (log(rest) - (a.s > 0.0f ? log_wide(a.s) + kEx2Low - log_s : -INFINITY));
-        if (first) t.loss[row] = (float)(t.factor * (double)w * l);
+        for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        const float s = a.s + listed, to_mass = t.lse ? 1.0f : 1.0f / (float)mass;
+        double rest = t.lse ? 1.0 - mass : 0.0;
+        if (rest <= kLeastTail) rest = 0.0;
+        if (team.rank == 0 && !dead) {
+            const double log_s = log_sum(s), log_mass = t.lse ? 0.0 : log_wide((float)mass);
+            double l = 0.0;
+            for (uint32_t i = lane; i < t.k; i += 32) {
+                const double log_q = (double)val[i] * r.inv_t - shift - log_mass;
+                const float q = share[i] * to_mass;
+                if (q != 0.0f) l += (double)q * (log_q - (((double)sx[i] - (double)m) * r.inv_t - log_s));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (rest > 0.0) l += rest * (log(rest) - (a.s > 0.0f ? log_wide(a.s) + kEx2Low - log_s : -INFINITY));
+            if (first) t.loss[row] = (float)(t.factor * (double)w * l);
+        }
+        if (tid == 0) {
+            // k = loss scale / T, the gradient's factor w T loss scale = w k T^2
+            found.m = m;
+            found.to_mass = to_mass;
+            found.f = (float)((double)w * (double)r.k * t.factor);
+            found.total = t.lse ? (float)(mass + rest) : 1.0f;
+            found.of_s = found.total / s;
+            found.outside = a.s > 0.0f ? found.of_s - (float)rest / a.s : 0.0f;
+            found.dead = dead;
+        }
     }
+    if (!r.d && team.ranks == 1) {
+        if (tid == 0 && found.dead) t.loss[row] = 0.0f;
+        return;
+    }
+    __syncthreads();
+    if (found.dead) return nothing_to_learn();
     if (!r.d) return;
-    // k = loss scale / T, the gradient's factor w T loss scale = w k T^2
-    const float f = (float)((double)w * (double)r.k * t.factor);
-    const float outside = a.s > 0.0f ? (float)((double)total / (double)s - rest / (double)a.s) : 0.0f;
-    write_row<T, NT, false>(r, row, m, Coef{f * outside, 0.0f, 0.0f}, -1);
+    write_row<T, NT, kSums>(r, row, part, team.rank, team.ranks, found.m, Coef{found.f * found.outside, 0.0f, 0.0f}, -1, 0.0f);
     __syncthreads();                        // the list's classes are written again, with their own values
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
-    for (uint32_t i = threadIdx.x; i < t.k; i += NT) {
-        if (!leads(i)) continue;
+    for (uint32_t i = tid; i < t.k; i += NT) {
+        if (!mine(i) || !leads(i)) continue;
         float q = 0.0f;
         for (uint32_t o = i; o < (twice ? t.k : i + 1); ++o)
-            if (idx[o] == idx[i]) q += raw_q(o) * to_mass;
-        const float df = sx[i] - m, e = ex2(fmaf(df, r.c_hi, df * r.c_lo));
-        d[idx[i]] = from_f32<T>(f * (total * e / s - q));
+            if (idx[o] == idx[i]) q += share[o] * found.to_mass;
+        const float df = sx[i] - found.m, e = ex2(fmaf(df, r.c_hi, df * r.c_lo));
+        d[idx[i]] = from_f32<T>(found.f * (found.of_s * e - q));
     }
 }
 

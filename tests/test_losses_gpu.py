@@ -20,7 +20,7 @@ DT = {"f32": (torch.float32, sk.Precision.FP32), "f16": (torch.float16, sk.Preci
 INF = math.inf
 LOG2E = 1.4426950408889634
 # classes: one, fewer than a unit, around warps, blocks and units, odd, wide
-SIZES = [(3, 1), (5, 2), (4, 7), (64, 10), (9, 33), (3, 255), (2, 256), (7, 1000), (5, 1023), (3, 1025), (3, 4099), (2, 10007), (2, 32768), (1, 50021), (2, 131072), (1, 300001)]
+SIZES = [(3, 1), (5, 2), (4, 7), (64, 10), (9, 33), (3, 255), (2, 256), (7, 1000), (5, 1023), (3, 1025), (3, 4099), (2, 10007), (2, 32768), (1, 50021), (2, 131072), (1, 250001), (1, 950001)]
 
 
 def _rng(seed):
@@ -262,6 +262,8 @@ def test_distillation(gpu_ctx, rows, classes, kind):
     for n, (pad, offset, tau, k, tail, weighted) in enumerate(((0, 0, 1.0, 1, False, False), (3, 1, 2.0, 20, True, True), (-classes % 64, 5, 4.0, 64, False, True),
                                                                (1, 2, 1.0, 300, True, False))):
         k = min(k, classes)
+        if classes > losses.MAX_LIST_CLASSES:
+            continue
         x, g = _logits(rows, classes, pad, kind, offset, seed=n)
         idx, values = _teacher(rows, classes, k, g)
         idx[:, k - k // 3:] = -1                                     # unused entries
@@ -606,6 +608,23 @@ def test_same_bits_again_on_another_stream_and_recorded(gpu_ctx, classes, kind):
             assert torch.equal(a, b), n
     del graph
     other.close()
+
+
+def test_a_step_slot_takes_rows_of_any_width(gpu_ctx):
+    """Wide rows are shared by the blocks of a cluster, narrow ones are not: one slot, one sequence of kernels, other clusters."""
+    made = []
+    for classes in (10, 70001, 700, 131072, 33, 40009, 250001):
+        x, g = _logits(5, classes, 0, "f32")
+        calls = _calls(x, g, classes)
+        made.append((calls, {n: [t.clone() for t in f(gpu_ctx)] for n, f in calls.items()}))
+    for _ in range(2):
+        for calls, want in made:
+            with gpu_ctx.step_graph(2):
+                got = {n: f(gpu_ctx) for n, f in calls.items()}
+            gpu_ctx.synchronize()
+            for n in calls:
+                for a, b in zip(got[n], want[n]):
+                    assert torch.equal(a, b), n
 
 
 def test_two_graphs_of_preference_losses_at_once(gpu_ctx):
