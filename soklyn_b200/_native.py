@@ -140,11 +140,11 @@ _SIGS = {
                                              C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32]),
     "sk_output_error": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32,
                                   C.c_uint32, C.c_uint32, C.c_float]),
-    "sk_label_logprob": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.c_void_p, C.c_void_p, C.c_void_p]),
-    "sk_label_logprob_backward": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.c_void_p, C.c_void_p, C.c_void_p]),
-    "sk_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkDistill)]),
-    "sk_policy_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkPolicy)]),
-    "sk_preference_loss": (C.c_int, [C.c_void_p, C.POINTER(SkLogits), C.POINTER(SkPreference)]),
+    "sk_label_logprob": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_label_logprob_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_distill_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_policy_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "sk_preference_loss": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "sk_output_gradient": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float]),
     "sk_hidden_error": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.POINTER(SkDense), C.c_uint32, C.c_uint32]),
     "sk_backward_update": (C.c_int, [C.c_void_p, C.POINTER(SkDense), C.c_void_p, C.c_uint32, C.c_uint32,

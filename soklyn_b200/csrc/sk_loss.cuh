@@ -376,10 +376,11 @@ template <typename T, int SUMS> __device__ __forceinline__ float gradient_of(flo
     return ex2(t) * (SUMS ? fmaf(k.b, SUMS == kMasked ? fmaxf(t, -200.0f) : t, k.a) : k.a);
 }
 template <typename T, int SUMS> __device__ __forceinline__ void gradient_unit(Unit<T> &q, const Rows &r, float m, const Coef &k) {
+    const f32x2 less = pair(-m, -m), hi = pair(r.c_hi, r.c_hi), ka = pair(k.a, k.a), kb = pair(k.b, k.b);
 #pragma unroll
     for (int i = 0; i < Unit<T>::V / 2; ++i) {
-        const float2 x = halves(q.get(i));
-        q.set(i, pair(gradient_of<T, SUMS>(x.x, r, m, k), gradient_of<T, SUMS>(x.y, r, m, k)));
+        const f32x2 d = add2(q.get(i), less), t = sizeof(T) == 4 ? fma2(d, hi, mul2(d, pair(r.c_lo, r.c_lo))) : mul2(d, hi);
+        q.set(i, mul2(ex2_2(t), SUMS ? fma2(kb, SUMS == kMasked ? floor2(t) : t, ka) : ka));
     }
 }
 
@@ -738,7 +739,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(Pairs p) {
 // d = k g (1[j = l] - p_j) from the kept maximum and sum. A row without a sum got no log-probability.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) sequence_gradient_kernel(Rows r, const int32_t *labels, const Kept *kept) {
-    const uint32_t row = blockIdx.x;
+    const uint32_t row = r.rows - 1 - blockIdx.x;       // the rows read last are still in the L2 cache
     grid_ready();
     const Kept k = kept[row];
     if (k.s == 0.0f || k.g == 0.0f) {
@@ -774,7 +775,7 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
 // which are listed, and these count as -inf where the row is summed; they are written by themselves behind the rest of the
 // gradient. Setting its bit also tells an entry whether its class was given before; the masses then add at the class.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT) distill_kernel(Rows r, Distill t) {
+__global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill t) {
     constexpr uint32_t V = Unit<T>::V;
     extern __shared__ uint32_t bits[];
     __shared__ typename Team<NT>::Shared shared;
@@ -787,6 +788,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(Rows r, Distill t) {
     grid_ready();
     const T *x = reinterpret_cast<const T *>(r.x) + (size_t)row * r.cols;
     const float w = t.weights ? t.weights[row] : 1.0f;
+    const int32_t early = tid < t.k ? t.indices[(size_t)row * t.k + tid] : -1;      // the longest chain of loads starts first
     auto nothing_to_learn = [&] {
         team.leave();
         if (first) t.loss[row] = 0.0f;
@@ -797,7 +799,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(Rows r, Distill t) {
     const uint32_t words = ((part.units + 2) * V + 31) / 32;
     for (uint32_t i = tid; i < words; i += NT) bits[i] = 0;
     for (uint32_t i = tid; i < t.k; i += NT) {
-        int32_t c = t.indices[(size_t)row * t.k + i];
+        int32_t c = i == tid ? early : t.indices[(size_t)row * t.k + i];
         if (c >= 0 && (uint32_t)c >= r.classes) { if (team.rank == 0) atomicOr(r.err, kErrList); c = -1; }
         idx[i] = c;
         val[i] = c >= 0 ? teacher_value(t, (size_t)row * t.k + i) : -INFINITY;

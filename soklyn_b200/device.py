@@ -13,9 +13,13 @@ import ctypes as C
 import torch
 
 from . import _native, log
-from ._native import SkDense, SkDistill, SkLogits, SkOptim, SkPolicy, SkPreference
+from ._native import SkDense, SkOptim
 from .core import SK_DTYPE, Tensor
 from .function import Activation, LossFunc, Normalisation, Optimiser, Precision
+
+
+# handle of torch's current stream on a device
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _optim(o: Optimiser) -> SkOptim:
@@ -120,28 +124,32 @@ class GpuContext:
         finally:
             self.step_keeps = keeps
 
-    def new_buffer(self, shape, dtype: torch.dtype) -> torch.Tensor:
+    def is_foreign(self) -> bool:
+        """Whether torch's current stream is another one than this context's."""
+        return _current_stream(self.device.index) != self.stream.cuda_stream
+
+    def new_buffer(self, shape, dtype: torch.dtype, foreign: bool) -> torch.Tensor:
         """Uninitialised memory of this context's stream; inside a step graph it is kept until the step has been launched."""
         if self.step_keeps is not None:
             self._check(self.lib.sk_step_allocations(self.handle, 1))
             try:
-                t = self._empty(shape, dtype)
+                t = self._empty(shape, dtype, foreign)
             finally:
                 self._check(self.lib.sk_step_allocations(self.handle, 0))
             self.step_keeps.append(t)
             return t
-        return self._empty(shape, dtype)
+        return self._empty(shape, dtype, foreign)
 
-    def _empty(self, shape, dtype):
-        if torch.cuda.current_stream(self.device) == self.stream:
+    def _empty(self, shape, dtype, foreign):
+        if not foreign:
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(self.stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
-    def uses(self, tensors):
+    def uses(self, tensors, foreign: bool):
         """These tensors are read or written by calls made so far: memory that another stream owns is not handed out
         again before they are through, and that of a recorded step not before it is launched."""
-        if torch.cuda.current_stream(self.device) != self.stream:
+        if foreign:
             for t in tensors:
                 t.record_stream(self.stream)
         if self.step_keeps is not None:
@@ -221,21 +229,22 @@ class GpuContext:
         self._check(self.lib.sk_output_gradient(self.handle, C.byref(layer.desc()), d_out.ptr(), d_out.rows(), batch_size,
                                                 batch_size if batch_stat is None else batch_stat, grad_scale))
 
-    # -- losses over rows of logits (no counterpart in the reference); arguments are checked by soklyn_b200/losses.py --
-    def gpu_label_logprob(self, logits: SkLogits, labels: int, logp: int, entropy: "int | None"):
-        self._check(self.lib.sk_label_logprob(self.handle, C.byref(logits), labels, logp, entropy))
+    # -- losses over rows of logits (no counterpart in the reference); soklyn_b200/losses.py checks the arguments and packs
+    # the descriptors --
+    def gpu_label_logprob(self, logits: bytes, labels: int, logp: int, entropy: int):
+        self._check(self.lib.sk_label_logprob(self.handle, logits, labels, logp, entropy))
 
-    def gpu_label_logprob_backward(self, logits: SkLogits, labels: int, d_logp: int, d_entropy: "int | None"):
-        self._check(self.lib.sk_label_logprob_backward(self.handle, C.byref(logits), labels, d_logp, d_entropy))
+    def gpu_label_logprob_backward(self, logits: bytes, labels: int, d_logp: int, d_entropy: int):
+        self._check(self.lib.sk_label_logprob_backward(self.handle, logits, labels, d_logp, d_entropy))
 
-    def gpu_distill_loss(self, logits: SkLogits, teacher: SkDistill):
-        self._check(self.lib.sk_distill_loss(self.handle, C.byref(logits), C.byref(teacher)))
+    def gpu_distill_loss(self, logits: bytes, teacher: bytes):
+        self._check(self.lib.sk_distill_loss(self.handle, logits, teacher))
 
-    def gpu_policy_loss(self, logits: SkLogits, policy: SkPolicy):
-        self._check(self.lib.sk_policy_loss(self.handle, C.byref(logits), C.byref(policy)))
+    def gpu_policy_loss(self, logits: bytes, policy: bytes):
+        self._check(self.lib.sk_policy_loss(self.handle, logits, policy))
 
-    def gpu_preference_loss(self, logits: SkLogits, preference: SkPreference):
-        self._check(self.lib.sk_preference_loss(self.handle, C.byref(logits), C.byref(preference)))
+    def gpu_preference_loss(self, logits: bytes, preference: bytes):
+        self._check(self.lib.sk_preference_loss(self.handle, logits, preference))
 
     def gpu_hidden_layer_error(self, cur, nxt, batch_size: int, batch_stat: int | None = None):
         self.check_tile_dim(cur.precision)

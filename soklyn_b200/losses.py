@@ -13,8 +13,8 @@ reported by the next `GpuContext.synchronize()` as `log.IndexOutOfRange`.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
 from enum import Enum
 from typing import NamedTuple, Optional
@@ -22,7 +22,6 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import log
-from ._native import SkDistill, SkLogits, SkPolicy, SkPreference
 from .core import SK_DTYPE, Tensor
 
 MAX_LIST = 512                # entries of a teacher's list
@@ -85,49 +84,65 @@ class PreferenceLoss(NamedTuple):
     d_logits: Optional[Tensor]
 
 
+# The descriptors of include/soklyn_b200.h, packed (a third of the time that ctypes structures of so many fields take)
+_LOGITS = struct.Struct("@IIIIPPff")
+_DISTILL = struct.Struct("@PPIIPPP")
+_POLICY = struct.Struct("@PPPPPffffPPPP")
+_PREFERENCE = struct.Struct("@PPIIIPPfffPPPPP")
+
+
 class _Call:
     """Checked logits of one call, the tensors it reads, and its outputs, allocated on the context's stream."""
 
+    __slots__ = ("context", "device", "rows", "cols", "classes", "data", "precision", "temperature", "grad_scale", "used", "foreign")
+
     def __init__(self, context, logits: Tensor, classes, temperature, grad_scale=1.0):
-        if logits.data.dim() != 2:
-            raise log.InvalidConfiguration(f"Logits must have two dimensions, not {logits.data.dim()}.")
+        data = logits.data
+        if data.dim() != 2:
+            raise log.InvalidConfiguration(f"Logits must have two dimensions, not {data.dim()}.")
         self.context, self.device = context, context.device
-        self.rows, self.cols = logits.data.shape
-        classes = self.cols if classes is None else classes
-        if self.cols == 0 or classes < 1:
+        self.rows, self.cols = rows, cols = data.shape
+        if classes is None:
+            classes = cols
+        if cols == 0 or classes < 1:
             raise log.InvalidConfiguration("Input or output size cannot be 0.")
-        if classes > self.cols:
-            raise log.MismatchedDimensions("classes vs logit columns", self.cols, classes)
+        if classes > cols:
+            raise log.MismatchedDimensions("classes vs logit columns", cols, classes)
+        if max(rows, cols) > 1 << 30:
+            raise log.AllocationLimitExceeded(max(rows, cols), 1 << 30, "rows or columns of logits")
         if not 1e-4 <= temperature <= 1e4:
             raise log.InvalidConfiguration(f"Temperature {temperature} must lie between 1e-4 and 1e4.")
         if not math.isfinite(grad_scale):
             raise log.InvalidConfiguration("The gradient scale must be finite.")
-        self.logits, self.classes = logits, classes
-        self.used = [self._here(logits.data, "logits")]
-        self.desc = SkLogits(SK_DTYPE[logits.precision], self.rows, self.cols, classes, logits.data.data_ptr(), None,
-                             temperature, grad_scale)
+        self.data, self.precision, self.classes, self.temperature, self.grad_scale = data, logits.precision, classes, temperature, grad_scale
+        self.used = []
+        self._use(data, "logits")
+        self.foreign = None
 
-    def _here(self, t: torch.Tensor, name: str) -> torch.Tensor:
+    def _use(self, t: torch.Tensor, name: str) -> int:
         if t.device != self.device:
             raise log.InvalidConfiguration(f"{name} lives on {t.device}, the context on {self.device}.")
         if not t.is_contiguous():
             raise log.InvalidConfiguration(f"{name} must be contiguous.")
-        return t
-
-    def vector(self, t, name: str, length, dtype=torch.float32):
-        """Address of a vector (or matrix) that the call reads; None stays None."""
-        if t is None:
-            return None
-        t = self._here(t.data if isinstance(t, Tensor) else t, name)
-        if t.dtype != dtype:
-            raise log.InvalidConfiguration(f"{name} must be {dtype}, not {t.dtype}.")
-        if t.numel() != length:
-            raise log.MismatchedDimensions(name, length, t.numel())
         self.used.append(t)
         return t.data_ptr()
 
+    def vector(self, t, name: str, length, dtype=torch.float32) -> int:
+        """Address of a vector (or matrix) that the call reads; 0 for None."""
+        if t is None:
+            return 0
+        if isinstance(t, Tensor):
+            t = t.data
+        if t.dtype is not dtype:
+            raise log.InvalidConfiguration(f"{name} must be {dtype}, not {t.dtype}.")
+        if t.numel() != length:
+            raise log.MismatchedDimensions(name, length, t.numel())
+        return self._use(t, name)
+
     def new(self, *shape, dtype=torch.float32) -> torch.Tensor:
-        return self.context.new_buffer(shape, dtype)
+        if self.foreign is None:
+            self.foreign = self.context.is_foreign()
+        return self.context.new_buffer(shape, dtype, self.foreign)
 
     def gradient(self, wanted: bool, out: "Tensor | None") -> "Tensor | None":
         """The Tensor the gradient goes to: a new one, or `out`, which may be the logits themselves."""
@@ -136,19 +151,20 @@ class _Call:
                 raise log.InvalidConfiguration("A gradient tensor was given, but no gradient asked for.")
             return None
         if out is None:
-            out = Tensor(self.new(self.rows, self.cols, dtype=self.logits.data.dtype), self.logits.precision, take_id=False)
-        else:
-            self._here(out.data, "out")
-            if out.precision != self.logits.precision:
-                raise log.UnsupportedTypeCast(out.precision, self.logits.precision)
-            if tuple(out.data.shape) != (self.rows, self.cols):
-                raise log.MismatchedDimensions("gradient elements", self.rows * self.cols, out.len())
-            self.used.append(out.data)
-        self.desc.d_logits = out.data.data_ptr()
+            return Tensor(self.new(self.rows, self.cols, dtype=self.data.dtype), self.precision, False)
+        if out.precision != self.precision:
+            raise log.UnsupportedTypeCast(out.precision, self.precision)
+        if tuple(out.data.shape) != (self.rows, self.cols):
+            raise log.MismatchedDimensions("gradient elements", self.rows * self.cols, out.len())
+        self._use(out.data, "out")
         return out
 
+    def logits(self, d: "Tensor | None") -> bytes:
+        return _LOGITS.pack(SK_DTYPE[self.precision], self.rows, self.cols, self.classes, self.data.data_ptr(),
+                            0 if d is None else d.data.data_ptr(), self.temperature, self.grad_scale)
+
     def done(self):
-        self.context.uses(self.used)
+        self.context.uses(self.used, self.foreign)
 
 
 def label_logprob(context, logits: Tensor, labels: torch.Tensor, *, temperature: float = 1.0, classes: "int | None" = None,
@@ -157,7 +173,7 @@ def label_logprob(context, logits: Tensor, labels: torch.Tensor, *, temperature:
     call = _Call(context, logits, classes, temperature)
     at = call.vector(labels, "labels", call.rows, torch.int32)
     logp, ent = call.new(call.rows), call.new(call.rows) if entropy else None
-    context.gpu_label_logprob(call.desc, at, logp.data_ptr(), ent.data_ptr() if entropy else None)
+    context.gpu_label_logprob(call.logits(None), at, logp.data_ptr(), ent.data_ptr() if entropy else 0)
     call.done()
     return LabelLogprob(logp, ent)
 
@@ -166,12 +182,12 @@ def label_logprob_backward(context, logits: Tensor, labels: torch.Tensor, d_logp
                            classes: "int | None" = None, grad_scale: float = 1.0, out: "Tensor | None" = None) -> Tensor:
     """Gradient of the logits from the gradients of label_logprob's outputs."""
     call = _Call(context, logits, classes, temperature, grad_scale)
-    at = call.vector(labels, "labels", call.rows, torch.int32)
-    d_logp, d_entropy = call.vector(d_logp, "d_logp", call.rows), call.vector(d_entropy, "d_entropy", call.rows)
     if d_logp is None:
         raise log.InvalidConfiguration("The gradient of the log-probabilities is missing.")
+    at = call.vector(labels, "labels", call.rows, torch.int32)
+    d_logp, d_entropy = call.vector(d_logp, "d_logp", call.rows), call.vector(d_entropy, "d_entropy", call.rows)
     d = call.gradient(True, out)
-    context.gpu_label_logprob_backward(call.desc, at, d_logp, d_entropy)
+    context.gpu_label_logprob_backward(call.logits(d), at, d_logp, d_entropy)
     call.done()
     return d
 
@@ -186,7 +202,7 @@ def distill_loss(context, logits: Tensor, indices: torch.Tensor, values, config:
     logits there, `teacher_lse` the log-sum-exp of all its logits / temperature where the mass outside the list counts."""
     call = _Call(context, logits, classes, config.temperature, grad_scale)
     values = values.data if isinstance(values, Tensor) else values
-    if indices.dim() != 2 or tuple(values.shape) != tuple(indices.shape):
+    if indices.dim() != 2 or values.shape != indices.shape:
         raise log.InvalidConfiguration(f"Indices {tuple(indices.shape)} and values {tuple(values.shape)} of a teacher must both be [rows x k].")
     k = indices.shape[1]
     if not 1 <= k <= MAX_LIST:
@@ -195,12 +211,11 @@ def distill_loss(context, logits: Tensor, indices: torch.Tensor, values, config:
         raise log.AllocationLimitExceeded(call.classes, MAX_LIST_CLASSES, "classes of a distillation")
     if values.dtype not in _VALUES:
         raise log.InvalidConfiguration(f"Teacher values must be f32, f16 or bf16, not {values.dtype}.")
-    t = SkDistill(call.vector(indices, "teacher indices", call.rows * k, torch.int32),
-                  call.vector(values, "teacher values", call.rows * k, values.dtype), _VALUES[values.dtype], k,
-                  call.vector(teacher_lse, "teacher_lse", call.rows), call.vector(weights, "weights", call.rows))
-    loss, d = call.new(call.rows), call.gradient(gradient, out)
-    t.loss = loss.data_ptr()
-    context.gpu_distill_loss(call.desc, t)
+    n = call.rows
+    read = (call.vector(indices, "teacher indices", n * k, torch.int32), call.vector(values, "teacher values", n * k, values.dtype),
+            _VALUES[values.dtype], k, call.vector(teacher_lse, "teacher_lse", n), call.vector(weights, "weights", n))
+    loss, d = call.new(n), call.gradient(gradient, out)
+    context.gpu_distill_loss(call.logits(d), _DISTILL.pack(*read, loss.data_ptr()))
     call.done()
     return DistillLoss(loss, d)
 
@@ -210,24 +225,24 @@ def policy_loss(context, logits: Tensor, actions: torch.Tensor, logp_old, advant
                 out: "Tensor | None" = None) -> PolicyLoss:
     """Clipped policy loss of each row's action, with a KL term to a reference policy and an entropy bonus."""
     call = _Call(context, logits, classes, config.temperature, grad_scale)
-    if not (0.0 <= config.clip_low <= 1.0 and config.clip_high >= 0.0):
-        raise log.InvalidConfiguration(f"Clip range {config.clip_low} below and {config.clip_high} above 1.")
-    if not (math.isfinite(config.kl_coeff) and math.isfinite(config.entropy_coeff)):
+    low, high, beta, eta = config.clip_low, config.clip_high, config.kl_coeff, config.entropy_coeff
+    if not (0.0 <= low <= 1.0 and high >= 0.0):
+        raise log.InvalidConfiguration(f"Clip range {low} below and {high} above 1.")
+    if not (math.isfinite(beta) and math.isfinite(eta)):
         raise log.InvalidConfiguration("Policy coefficients must be finite.")
-    if config.kl_coeff != 0.0 and logp_ref is None:
+    if beta != 0.0 and logp_ref is None:
         raise log.InvalidConfiguration("A KL term needs the reference's log-probabilities.")
     if logp_old is None or advantages is None:
         raise log.InvalidConfiguration("Old log-probabilities or advantages are missing.")
     n = call.rows
-    p = SkPolicy(call.vector(actions, "actions", n, torch.int32), call.vector(logp_old, "logp_old", n),
-                 call.vector(advantages, "advantages", n), call.vector(logp_ref, "logp_ref", n), call.vector(weights, "weights", n),
-                 config.clip_low, config.clip_high, config.kl_coeff, config.entropy_coeff)
-    loss, logp, kl, entropy = call.new(4, n).unbind()
-    p.loss, p.logp, p.kl, p.entropy = loss.data_ptr(), logp.data_ptr(), kl.data_ptr(), entropy.data_ptr()
+    read = (call.vector(actions, "actions", n, torch.int32), call.vector(logp_old, "logp_old", n), call.vector(advantages, "advantages", n),
+            call.vector(logp_ref, "logp_ref", n), call.vector(weights, "weights", n))
+    of_rows = call.new(4, n)
     d = call.gradient(gradient, out)
-    context.gpu_policy_loss(call.desc, p)
+    at = of_rows.data_ptr()
+    context.gpu_policy_loss(call.logits(d), _POLICY.pack(*read, low, high, beta, eta, at, at + 4 * n, at + 8 * n, at + 12 * n))
     call.done()
-    return PolicyLoss(loss, logp, kl, entropy, d)
+    return PolicyLoss(*of_rows.unbind(), d)
 
 
 def preference_loss(context, logits: Tensor, labels: torch.Tensor, offsets: torch.Tensor,
@@ -241,20 +256,19 @@ def preference_loss(context, logits: Tensor, labels: torch.Tensor, offsets: torc
         raise log.InvalidConfiguration("Beta and target margin must be finite.")
     if not 0.0 <= config.label_smoothing <= 1.0:
         raise log.InvalidConfiguration(f"Label smoothing {config.label_smoothing} must lie between 0 and 1.")
-    if config.label_smoothing != 0.0 and config.form != PreferenceForm.Sigmoid:
+    if config.label_smoothing != 0.0 and config.form is not PreferenceForm.Sigmoid:
         raise log.InvalidConfiguration("Only the sigmoid form takes label smoothing.")
     if offsets.numel() % 2 != 1:
         raise log.InvalidConfiguration(f"Pairs of sequences have an odd number of offsets, not {offsets.numel()}.")
     n, pairs = call.rows, offsets.numel() // 2
-    p = SkPreference(call.vector(labels, "labels", n, torch.int32), call.vector(offsets, "offsets", 2 * pairs + 1, torch.int32),
-                     pairs, config.form.value, int(config.average), call.vector(logp_ref, "logp_ref", 2 * pairs),
-                     call.vector(weights, "weights", pairs), config.beta, config.label_smoothing, config.target_margin)
-    of_pairs, of_rows = call.new(4 * pairs), call.new(5 * n)
-    loss, margin, logp = of_pairs.split((pairs, pairs, 2 * pairs))
-    scratch, row_logp = of_rows.split((4 * n, n))
-    p.loss, p.margin, p.logp = loss.data_ptr(), margin.data_ptr(), logp.data_ptr()
-    p.row_logp, p.scratch = row_logp.data_ptr(), scratch.data_ptr()
+    read = (call.vector(labels, "labels", n, torch.int32), call.vector(offsets, "offsets", 2 * pairs + 1, torch.int32), pairs,
+            config.form.value, bool(config.average), call.vector(logp_ref, "logp_ref", 2 * pairs), call.vector(weights, "weights", pairs),
+            config.beta, config.label_smoothing, config.target_margin)
+    own = call.new(5 * n + 4 * pairs)       # scratch [4 n], row_logp [n], loss, margin [pairs], logp [2 pairs]
     d = call.gradient(gradient, out)
-    context.gpu_preference_loss(call.desc, p)
+    at = own.data_ptr()
+    of_pairs = at + 20 * n
+    context.gpu_preference_loss(call.logits(d), _PREFERENCE.pack(*read, of_pairs, of_pairs + 4 * pairs, of_pairs + 8 * pairs, at + 16 * n, at))
     call.done()
+    _, row_logp, loss, margin, logp = own.split_with_sizes((4 * n, n, pairs, pairs, 2 * pairs))
     return PreferenceLoss(loss, margin, logp, row_logp, d)

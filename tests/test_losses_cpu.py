@@ -115,3 +115,5 @@ def test_descriptor_layouts_match_the_header():
     import ctypes as C
     assert C.sizeof(_native.SkLogits) == 40 and C.sizeof(_native.SkDistill) == 48
     assert C.sizeof(_native.SkPolicy) == 88 and C.sizeof(_native.SkPreference) == 104
+    # the packed forms, up to the padding behind the last field
+    assert losses._LOGITS.size == 40 and losses._DISTILL.size == 48 and losses._POLICY.size == 88 and losses._PREFERENCE.size == 104
