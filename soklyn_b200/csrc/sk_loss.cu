@@ -63,20 +63,17 @@ int make_rows(sk_ctx *c, const sk_logits *x, bool need_gradient, loss::Rows *out
 
 // Threads of a block and blocks of a cluster for a row; the reasons stand beside Team. `twice`: the row is read again.
 constexpr size_t kWarpRow = 32 * loss::kWarpUnits * 16, kPerThread = 256;
-#ifndef SK_MAXT
-#define SK_MAXT 256
-#endif
-constexpr uint32_t kMostThreads = SK_MAXT;
+constexpr uint32_t kMostThreads = 256;
 struct RowPlan { uint32_t threads, ranks; };
 RowPlan plan_row(const sk_ctx *c, const loss::Rows &r, size_t one, bool twice) {
-    const size_t bytes = (size_t)r.classes * one, sms = (size_t)c->num_sms;
+    const size_t bytes = (size_t)r.classes * one, rows = r.rows, sms = (size_t)c->num_sms;
     if (bytes <= kWarpRow) return RowPlan{32, 1};
     RowPlan plan{64, 1};
     while (plan.threads < kMostThreads && bytes > plan.threads * kPerThread) plan.threads *= 2;
     while (twice && plan.ranks < loss::kMaxCluster && bytes > plan.ranks * plan.threads * kPerThread) plan.ranks *= 2;
     // few rows: more threads for each, then more blocks, down to 32 bytes per thread
-    while (plan.threads < kMostThreads && r.rows * plan.threads < sms * 1024 && bytes >= plan.threads * 64) plan.threads *= 2;
-    while (plan.ranks < loss::kMaxCluster && r.rows * plan.ranks * 2 <= sms && bytes >= plan.ranks * plan.threads * 64) plan.ranks *= 2;
+    while (plan.threads < kMostThreads && rows * plan.threads < sms * 1024 && bytes >= plan.threads * 64) plan.threads *= 2;
+    while (plan.ranks < loss::kMaxCluster && rows * plan.ranks * 2 <= sms && bytes >= plan.ranks * plan.threads * 64) plan.ranks *= 2;
     return plan;
 }
 template <typename T, class Op, int SUMS, bool GRAD> cudaError_t launch_rows(sk_ctx *c, const loss::Rows &r, const Op &op) {

@@ -51,12 +51,11 @@ __device__ __forceinline__ double log_wide(float s) {
     if (f < 0.70710678f) { f *= 2.0f; --e; }
     return (double)e * 0.69314718055994531 + (double)logf(f);
 }
-// log of a sum of ex2 results of which the largest is 1. The instruction's results are 5.0e-8 too small on average
-// (measured over [-32, 0), the same in every octave; 1.4e-7 at most, and exact for 1): the same sign in every row, which
-// the sum over a sequence would not average out. It made 8e-6 of a preference margin of sequences that differ by
-// hundreds of rows.
-constexpr double kEx2Low = 5.0e-8;
-__device__ __forceinline__ double log_sum(float s) { return log_wide(s) + (double)((float)kEx2Low * (1.0f - __fdividef(1.0f, s))); }
+// What ex2 lacks: its results are 5.1e-8 too small on average (measured over [-32, 0), weighted by size, the same in every
+// octave; 1.4e-7 at most), and exact for the exponent 0 of a thread's own maximum. It is the same sign in every row, which
+// the sum over a sequence does not average out: it made 8e-6 of a preference margin of sequences that differ by hundreds
+// of rows. A thread's sum is lifted by it.
+constexpr float kEx2Low = 5.0e-8f;
 
 // The largest of a warp's values, in every lane; one instruction on sm_100a. NaN only if all are.
 __device__ __forceinline__ float max_of_warp(float v) {
@@ -180,40 +179,65 @@ template <typename T> __device__ __forceinline__ Unit<T> part_unit(const T *p, u
 }
 
 // ---- row statistics ------------------------------------------------------------------------
-struct Stat { float m, s, u; };             // maximum, sum e, sum e t2 (t2 = t log2 e), relative to m
+// Of the classes that a thread has seen: the maximum, sum e and sum e t2 (t2 = t log2 e), relative to it.
+struct Share { float m, s, u; };
+// Of a part of a row: instead of sum e what it is beyond the 1 of one class at the maximum. Of a label that is nearly
+// certain, log p is the log1p of that, of which 1 + it would keep the f32 places of 1 only.
+struct Stat {
+    float m, more, u;
+    __device__ __forceinline__ float s() const { return m == -INFINITY ? more : 1.0f + more; }      // no class: 0 (or NaN)
+    __device__ __forceinline__ double log_s() const { return more < 0.4f ? (double)log1pf(more) : log_wide(1.0f + more); }
+};
 
 // What is summed beside e. kSums: nothing; the exponent is the product with both parts of log2(e) / T. kEntropy: e t2 as
 // well, from which the second part's effect on s follows at once (with_low), so that one product is enough. A class at
 // -inf makes NaN of e t2 = 0 * -inf; such a row is taken again with kMasked, which bounds t2 at -200, where e is 0 already.
 enum Sums : int { kSums = 0, kEntropy = 1, kMasked = 2 };
-// (s, u) of a partial sum relative to m, seen from the larger maximum `to`. An exponent beyond f32 makes NaN of u as one
-// class's does, unless that is bounded.
-template <int SUMS> __device__ __forceinline__ void rescale(Stat &a, float to, float c) {
-    if (a.m == -INFINITY) { a.m = to; return; }   // holds no class (or only NaN, which s keeps)
-    const float d = (a.m - to) * c, f = ex2(d);
-    if (SUMS) a.u = f * fmaf(SUMS == kMasked ? fmaxf(d, -200.0f) : d, a.s, a.u);
-    a.s *= f;
-    a.m = to;
+// 2^t for t <= 0, from its power series in the fraction: right to a rounding of either sign. With ex2 for the factors of
+// partial sums, even lifted, up to 1.1e-7 of a row's sum was left; with this 3e-8.
+__device__ __forceinline__ float pow2(float t) {
+    if (t < -126.0f) return 0.0f;
+    const float n = rintf(t), r = (t - n) * kLn2, r2 = r * r;
+    const float upper = fmaf(r2, fmaf(r, 1.0f / 5040.0f, 1.0f / 720.0f), fmaf(r, 1.0f / 120.0f, 1.0f / 24.0f));
+    const float p = 1.0f + fmaf(r2 * r2, upper, fmaf(r2, fmaf(r, 1.0f / 6.0f, 0.5f), r));
+    return p * __int_as_float(((int)n + 127) << 23);
+}
+// log2 of the factor that takes sums relative to m to the larger maximum `to`. Beyond f32 it makes NaN of u as one class's
+// does, unless that is bounded.
+template <int SUMS> __device__ __forceinline__ float factor_log(float m, float to, float c_hi, float c_lo) {
+    const float by = m - to;
+    return SUMS == kSums ? fmaf(by, c_hi, by * c_lo) : by * c_hi;
+}
+template <int SUMS> __device__ __forceinline__ float moved_u(float u, float s, float d, float f) {
+    return f * fmaf(SUMS == kMasked ? fmaxf(d, -200.0f) : d, s, u);
 }
 
 __device__ __forceinline__ f32x2 floor2(f32x2 t) { const float2 v = halves(t); return pair(fmaxf(v.x, -200.0f), fmaxf(v.y, -200.0f)); }
 
-template <typename T, int U, int SUMS> __device__ __forceinline__ void accumulate(Stat &a, const Unit<T> (&q)[U], float c_hi, float c_lo) {
+template <typename T, int U, int SUMS> __device__ __forceinline__ void accumulate(Share &a, const Unit<T> (&q)[U], float c_hi, float c_lo) {
     float mx = q[0].max();
 #pragma unroll
     for (int k = 1; k < U; ++k) mx = fmaxf(mx, q[k].max());
-    if (mx > a.m) rescale<SUMS>(a, mx, c_hi);
+    if (mx > a.m) {
+        if (a.m != -INFINITY) {
+            const float d = factor_log<SUMS>(a.m, mx, c_hi, c_lo), f = ex2(d);
+            if (SUMS) a.u = moved_u<SUMS>(a.u, a.s, d, f);
+            a.s *= fmaf(f, kEx2Low, f);
+        }
+        a.m = mx;
+    }
     const float ref = a.m == -INFINITY ? 0.0f : a.m;
     const f32x2 less = pair(-ref, -ref), hi = pair(c_hi, c_hi), lo = pair(c_lo, c_lo);
     f32x2 s = 0, u = 0;
 #pragma unroll
-    for (int k = 0; k < U; ++k)
+    for (int k = 0; k < U; ++k) {
 #pragma unroll
         for (int i = 0; i < Unit<T>::V / 2; ++i) {
             const f32x2 d = add2(q[k].get(i), less), t = SUMS == kSums ? fma2(d, hi, mul2(d, lo)) : mul2(d, hi), e = ex2_2(t);
             s = add2(s, e);
             if (SUMS) u = fma2(e, SUMS == kMasked ? floor2(t) : t, u);
         }
+    }
     const float2 ss = halves(s);
     a.s += ss.x + ss.y;
     if (SUMS) {
@@ -221,12 +245,35 @@ template <typename T, int U, int SUMS> __device__ __forceinline__ void accumulat
         a.u += us.x + us.y;
     }
 }
+// The statistics of n parts (a power of two), in every lane, in a fixed order; each group of n lanes holds the same parts.
+template <int SUMS> __device__ __forceinline__ Stat join(Stat a, uint32_t n, float c_hi, float c_lo) {
+    float m = a.m;
+    if (n == 32) m = max_of_warp(m);
+    else for (uint32_t o = n / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t keeps = __ffs(__ballot_sync(0xffffffffu, a.m == m)) - 1;     // the part whose 1 is left out
+    if (a.m != -INFINITY) {
+        const float d = factor_log<SUMS>(a.m, m, c_hi, c_lo), f = pow2(d);
+        if (SUMS) a.u = moved_u<SUMS>(a.u, 1.0f + a.more, d, f);
+        if ((threadIdx.x & (n - 1)) != keeps) a.more = fmaf(a.more, f, f);
+    }
+    a.m = m;
+    for (uint32_t o = n / 2; o > 0; o >>= 1) {
+        a.more += __shfl_xor_sync(0xffffffffu, a.more, o);
+        if (SUMS) a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+    }
+    return a;
+}
+// A warp's from the shares of its lanes, which are lifted by what ex2 lacks on the way.
+template <int SUMS> __device__ __forceinline__ Stat join_lanes(const Share &a, float c_hi, float c_lo) {
+    const float beyond = a.s - 1.0f;
+    return join<SUMS>(Stat{a.m, a.m == -INFINITY ? a.s : fmaf(beyond, kEx2Low, beyond), a.u}, 32, c_hi, c_lo);
+}
 // sum 2^(d (c_hi + c_lo)) = sum e (1 + ln2 d c_lo) up to 1e-12
-__device__ __forceinline__ void with_low(Stat &a, float c_hi, float c_lo) { a.s = fmaf(kLn2 * c_lo / c_hi, a.u, a.s); }
-__device__ __forceinline__ bool masked(const Stat &a) { return a.u != a.u && a.s == a.s; }
+__device__ __forceinline__ void with_low(Stat &a, float c_hi, float c_lo) { a.more = fmaf(kLn2 * c_lo / c_hi, a.u, a.more); }
+__device__ __forceinline__ bool masked(const Stat &a) { return a.u != a.u && a.more == a.more; }
 
 // A row all of whose classes are -inf has no distribution.
-__device__ __forceinline__ bool nothing(const Stat &a) { return a.m == -INFINITY && a.s == 0.0f; }
+__device__ __forceinline__ bool nothing(const Stat &a) { return a.m == -INFINITY && a.more == 0.0f; }
 
 // ---- who works on a row -----------------------------------------------------------------------------
 // A row of up to 4 KB is held by one warp in registers. Wider ones belong to a block, which reads them again for the
@@ -240,7 +287,7 @@ __device__ __forceinline__ bool nothing(const Stat &a) { return a.m == -INFINITY
 constexpr int kAhead = 4;                   // units of a thread whose loads are in flight together
 constexpr uint32_t kMaxCluster = 8;
 constexpr int kWarpUnits = 8;               // units of a lane of a row held by a warp
-struct alignas(16) Message { float m, s, u; int flag; };
+struct alignas(16) Message { float m, more, u; int flag; };
 
 // A block's part of a row: units [first, first + units) of its span, with the head before unit 0 and the tail behind the last.
 template <typename T> struct Part {
@@ -279,53 +326,35 @@ template <int NT> struct Team {
         __syncwarp();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    // The block's statistics from those of its threads, in every thread, in a fixed order.
-    template <int SUMS> __device__ __forceinline__ Stat merge(Stat a, float c) {
+    // The block's statistics from those of its threads, in every thread, in a fixed order. Every warp joins all the
+    // warps' parts, a lane to each: one after the other they took 10 % of a row of 64 KB.
+    template <int SUMS> __device__ __forceinline__ Stat merge(const Share &share, float c_hi, float c_lo) {
         Stat(&red)[NT / 32] = sh.red[merged++ & 1];      // the other one may still be read
-        rescale<SUMS>(a, max_of_warp(a.m), c);
-        a.s = warp_sum(a.s);
-        if (SUMS) a.u = warp_sum(a.u);
+        const Stat a = join_lanes<SUMS>(share, c_hi, c_lo);
         if (lane == 0) red[tid / 32] = a;
         __syncthreads();
-        Stat b[NT / 32], t{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < NT / 32; ++w) { b[w] = red[w]; t.m = fmaxf(t.m, b[w].m); }
-#pragma unroll
-        for (int w = 0; w < NT / 32; ++w) {
-            rescale<SUMS>(b[w], t.m, c);
-            t.s += b[w].s;
-            if (SUMS) t.u += b[w].u;
-        }
-        return t;
+        return join<SUMS>(red[lane % (NT / 32)], NT / 32, c_hi, c_lo);
     }
-    // The cluster's from those of its blocks, in rank order. All blocks of the cluster, the same number of times.
-    template <int SUMS> __device__ __forceinline__ Stat meet(const Stat &a, int flag, float c, int *any) {
+    // The cluster's from those of its blocks, in a fixed order. All blocks of the cluster, the same number of times.
+    template <int SUMS> __device__ __forceinline__ Stat meet(const Stat &a, int flag, float c_hi, float c_lo, int *any) {
         if (ranks == 1) { *any = flag; return a; }
         if (met == 0) cluster_wait();                    // every block runs: its shared memory may be written
         Message(&box)[kMaxCluster] = sh.box[met++ & 1];  // of the other one a block may still be reading
         if (tid < ranks) {
             const uint32_t at = tc::map_shared(tc::smem_u32(&box[rank]), tid);
-            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.s)), "r"(__float_as_uint(a.u)), "r"(flag) : "memory");
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(__float_as_uint(a.m)), "r"(__float_as_uint(a.more)), "r"(__float_as_uint(a.u)), "r"(flag) : "memory");
         }
         tc::cluster_sync();
-        Stat t{-INFINITY, 0.0f, 0.0f};
-        *any = 0;
-        for (uint32_t i = 0; i < ranks; ++i) t.m = fmaxf(t.m, box[i].m);
-        for (uint32_t i = 0; i < ranks; ++i) {
-            Stat b{box[i].m, box[i].s, box[i].u};
-            rescale<SUMS>(b, t.m, c);
-            t.s += b.s;
-            if (SUMS) t.u += b.u;
-            *any |= box[i].flag;
-        }
-        return t;
+        const Message &b = box[lane & (ranks - 1)];      // a lane to each again; ranks is a power of two
+        *any = __any_sync(0xffffffffu, b.flag);
+        return join<SUMS>(Stat{b.m, b.more, b.u}, ranks, c_hi, c_lo);
     }
     // A thread's share of the statistics of this block's part of the row at x. Units that do not fill a group are summed one
     // by one, the head and the tail by the form that takes places that are no classes. `leave` takes (unit, its place).
     template <typename T, int SUMS, class Leave>
-    __device__ __forceinline__ Stat scan(const T *x, const Part<T> &p, float c_hi, float c_lo, const Leave &leave) const {
+    __device__ __forceinline__ Share scan(const T *x, const Part<T> &p, float c_hi, float c_lo, const Leave &leave) const {
         constexpr uint32_t V = Part<T>::V;
-        Stat a{-INFINITY, 0.0f, 0.0f};
+        Share a{-INFINITY, 0.0f, 0.0f};
         for (uint32_t u = tid; u < p.units; u += NT * kAhead) {
             Unit<T> q[kAhead];
 #pragma unroll
@@ -460,9 +489,9 @@ struct LabelLogprob {
     }
     __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &, bool first) const {
         if (first) {
-            const double log_s = log_sum(a.s);
+            const double log_s = a.log_s();
             logp[row] = (float)log_prob(r, a, log_s, x);
-            if (entropy) entropy[row] = (float)(log_s - (double)(a.u / a.s * kLn2));
+            if (entropy) entropy[row] = (float)(log_s - (double)(a.u / a.s() * kLn2));
         }
         return Coef{0.0f, 0.0f, 0.0f};
     }
@@ -477,8 +506,8 @@ struct LabelLogprobBackward {
     static __device__ __forceinline__ int32_t label_of(const In &in) { return in.label; }
     __device__ __forceinline__ void skip(uint32_t) const {}
     __device__ __forceinline__ Coef finish(const Rows &r, uint32_t, const Stat &a, float, const In &in, bool) const {
-        const float f = r.k / a.s;
-        return Coef{f * (in.h * (a.u / a.s) - in.g), -f * in.h, r.k * in.g};
+        const float f = r.k / a.s();
+        return Coef{f * (in.h * (a.u / a.s()) - in.g), -f * in.h, r.k * in.g};
     }
 };
 
@@ -506,10 +535,10 @@ struct Policy {
         return p * d * d;
     }
     __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &in, bool first) const {
-        const double log_s = log_sum(a.s), lp = log_prob(r, a, log_s, x);
+        const double log_s = a.log_s(), lp = log_prob(r, a, log_s, x);
         const float w = in.w, adv = in.adv;
         const float rho = expf((float)(lp - (double)in.old));
-        const float d = ref ? (float)((double)in.ref - lp) : 0.0f, h = (float)(log_s - (double)(a.u / a.s * kLn2));
+        const float d = ref ? (float)((double)in.ref - lp) : 0.0f, h = (float)(log_s - (double)(a.u / a.s() * kLn2));
         const float plain = rho * adv, held = fminf(fmaxf(rho, lo), hi) * adv;
         const bool clipped = (adv > 0.0f && rho > hi) || (adv < 0.0f && rho < lo);
         float g = clipped ? 0.0f : -plain;
@@ -525,8 +554,8 @@ struct Policy {
             if (entropy) entropy[row] = h;
         }
         g *= w;
-        const float f = r.k / a.s, q = w * eta * kLn2;
-        return Coef{f * (-g - q * (a.u / a.s)), f * q, r.k * g};
+        const float f = r.k / a.s(), q = w * eta * kLn2;
+        return Coef{f * (-g - q * (a.u / a.s())), f * q, r.k * g};
     }
 };
 
@@ -551,9 +580,9 @@ struct SequenceLogprob {
     }
     __device__ __forceinline__ Coef finish(const Rows &r, uint32_t row, const Stat &a, float x, const In &, bool first) const {
         if (first) {
-            const double lp = log_prob(r, a, log_sum(a.s), x);
+            const double lp = log_prob(r, a, a.log_s(), x);
             row_logp[row] = (float)lp;
-            Kept k{a.m, a.s, 0.0f, 0.0f};
+            Kept k{a.m, a.s(), 0.0f, 0.0f};
             if (isfinite(lp)) k.low = (float)(lp - (double)(float)lp);
             kept[row] = k;
         }
@@ -581,13 +610,13 @@ __global__ void __launch_bounds__(NT) row_kernel(Rows r, Op op) {
     const float at = to_f32(x[label]);
     const Part<T> part(Span<T>(x, r.classes), team.rank, team.ranks);
     int any;
-    Stat a = team.template merge<SUMS>(team.template scan<T, SUMS>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi);
-    a = team.template meet<SUMS>(a, 0, r.c_hi, &any);
+    Stat a = team.template merge<SUMS>(team.template scan<T, SUMS>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi, r.c_lo);
+    a = team.template meet<SUMS>(a, 0, r.c_hi, r.c_lo, &any);
     bool again = false;
     if (SUMS == kEntropy && masked(a)) {
         again = true;
-        a = team.template merge<kMasked>(team.template scan<T, kMasked>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi);
-        a = team.template meet<kMasked>(a, 0, r.c_hi, &any);
+        a = team.template merge<kMasked>(team.template scan<T, kMasked>(x, part, r.c_hi, r.c_lo, LeaveNone()), r.c_hi, r.c_lo);
+        a = team.template meet<kMasked>(a, 0, r.c_hi, r.c_lo, &any);
     }
     if (SUMS) with_low(a, r.c_hi, r.c_lo);
     if (nothing(a)) return skip();
@@ -624,16 +653,13 @@ __global__ void __launch_bounds__(kThreads) warp_kernel(Rows r, Op op) {
     Stat a{-INFINITY, 0.0f, 0.0f};
     if (label >= 0) {
         at = to_f32(x[label]);
+        Share share{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < kWarpUnits; k += 2)
-            if (k * 32 < p.units) accumulate<T, 2, SUMS>(a, reinterpret_cast<const Unit<T>(&)[2]>(q[k]), r.c_hi, r.c_lo);
-        if (side) accumulate<T, 1, SUMS>(a, reinterpret_cast<const Unit<T>(&)[1]>(edge), r.c_hi, r.c_lo);
-        rescale<SUMS>(a, max_of_warp(a.m), r.c_hi);
-        a.s = warp_sum(a.s);
-        if (SUMS) {
-            a.u = warp_sum(a.u);
-            with_low(a, r.c_hi, r.c_lo);
-        }
+            if (k * 32 < p.units) accumulate<T, 2, SUMS>(share, reinterpret_cast<const Unit<T>(&)[2]>(q[k]), r.c_hi, r.c_lo);
+        if (side) accumulate<T, 1, SUMS>(share, reinterpret_cast<const Unit<T>(&)[1]>(edge), r.c_hi, r.c_lo);
+        a = join_lanes<SUMS>(share, r.c_hi, r.c_lo);
+        if (SUMS) with_low(a, r.c_hi, r.c_lo);
     }
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
     if (label < 0 || nothing(a)) {
@@ -827,9 +853,9 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
         if (mark)
 #pragma unroll
             for (int j = 0; j < (int)V; ++j) if (mark >> j & 1u) q.drop(j);
-    }), r.c_hi);
+    }), r.c_hi, r.c_lo);
     int any;
-    a = team.template meet<kSums>(a, twice, r.c_hi, &any);
+    a = team.template meet<kSums>(a, twice, r.c_hi, r.c_lo, &any);
     twice = any;
     auto leads = [&](uint32_t i) {          // the first entry of its class
         if (twice)
@@ -841,22 +867,22 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
         float best = -INFINITY, listed = 0.0f;
         for (uint32_t i = lane; i < t.k; i += 32) best = fmaxf(best, sx[i]);
         const float m = fmaxf(a.m, max_of_warp(best));
-        const bool dead = (!t.lse && (!some || top == -INFINITY)) || (m == -INFINITY && a.s == 0.0f);
-        rescale<kSums>(a, m, r.c_hi);
+        const bool dead = (!t.lse && (!some || top == -INFINITY)) || (m == -INFINITY && a.more == 0.0f);
+        const float outside = a.m == -INFINITY ? a.more : a.s() * pow2(factor_log<kSums>(a.m, m, r.c_hi, r.c_lo));
         double mass = 0.0;
         for (uint32_t i = lane; i < t.k; i += 32) {
-            const float d = sx[i] - m, e = ex2(fmaf(d, r.c_hi, d * r.c_lo));
+            const float d = sx[i] - m, e = pow2(fmaf(d, r.c_hi, d * r.c_lo));
             if (leads(i)) listed += e;
             mass += (double)share[i];
         }
         listed = warp_sum(listed);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-        const float s = a.s + listed, to_mass = t.lse ? 1.0f : 1.0f / (float)mass;
+        const float s = outside + listed, to_mass = t.lse ? 1.0f : 1.0f / (float)mass;
         double rest = t.lse ? 1.0 - mass : 0.0;
         if (rest <= kLeastTail) rest = 0.0;
         if (team.rank == 0 && !dead) {
-            const double log_s = log_sum(s), log_mass = t.lse ? 0.0 : log_wide((float)mass);
+            const double log_s = log_wide(s), log_mass = t.lse ? 0.0 : log_wide((float)mass);
             double l = 0.0;
             for (uint32_t i = lane; i < t.k; i += 32) {
                 const double log_q = (double)val[i] * r.inv_t - shift - log_mass;
@@ -865,7 +891,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (rest > 0.0) l += rest * (log(rest) - (a.s > 0.0f ? log_wide(a.s) + kEx2Low - log_s : -INFINITY));
+            if (rest > 0.0) l += rest * (log(rest) - (outside > 0.0f ? log_wide(outside) - log_s : -INFINITY));
             if (first) t.loss[row] = (float)(t.factor * (double)w * l);
         }
         if (tid == 0) {
@@ -875,7 +901,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             found.f = (float)((double)w * (double)r.k * t.factor);
             found.total = t.lse ? (float)(mass + rest) : 1.0f;
             found.of_s = found.total / s;
-            found.outside = a.s > 0.0f ? found.of_s - (float)rest / a.s : 0.0f;
+            found.outside = outside > 0.0f ? found.of_s - (float)rest / outside : 0.0f;
             found.dead = dead;
         }
     }

@@ -94,7 +94,7 @@ _PREFERENCE = struct.Struct("@PPIIIPPfffPPPPP")
 class _Call:
     """Checked logits of one call, the tensors it reads, and its outputs, allocated on the context's stream."""
 
-    __slots__ = ("context", "device", "rows", "cols", "classes", "data", "precision", "temperature", "grad_scale", "used", "foreign")
+    __slots__ = ("context", "device", "rows", "cols", "classes", "data", "precision", "temperature", "grad_scale", "used", "_foreign")
 
     def __init__(self, context, logits: Tensor, classes, temperature, grad_scale=1.0):
         data = logits.data
@@ -117,7 +117,7 @@ class _Call:
         self.data, self.precision, self.classes, self.temperature, self.grad_scale = data, logits.precision, classes, temperature, grad_scale
         self.used = []
         self._use(data, "logits")
-        self.foreign = None
+        self._foreign = None
 
     def _use(self, t: torch.Tensor, name: str) -> int:
         if t.device != self.device:
@@ -139,10 +139,13 @@ class _Call:
             raise log.MismatchedDimensions(name, length, t.numel())
         return self._use(t, name)
 
+    def foreign(self) -> bool:
+        if self._foreign is None:
+            self._foreign = self.context.is_foreign()
+        return self._foreign
+
     def new(self, *shape, dtype=torch.float32) -> torch.Tensor:
-        if self.foreign is None:
-            self.foreign = self.context.is_foreign()
-        return self.context.new_buffer(shape, dtype, self.foreign)
+        return self.context.new_buffer(shape, dtype, self.foreign())
 
     def gradient(self, wanted: bool, out: "Tensor | None") -> "Tensor | None":
         """The Tensor the gradient goes to: a new one, or `out`, which may be the logits themselves."""
@@ -164,7 +167,7 @@ class _Call:
                             0 if d is None else d.data.data_ptr(), self.temperature, self.grad_scale)
 
     def done(self):
-        self.context.uses(self.used, self.foreign)
+        self.context.uses(self.used, self.foreign())
 
 
 def label_logprob(context, logits: Tensor, labels: torch.Tensor, *, temperature: float = 1.0, classes: "int | None" = None,

@@ -522,6 +522,41 @@ def test_long_sequences_keep_their_margin(gpu_ctx):
 
 # ---- all of them ------------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes,tau", [(20, 0.7), (20, 1.0), (3000, 0.7), (3000, 1.0), (20000, 0.7)])
+def test_a_sequence_adds_no_bias_of_its_rows(gpu_ctx, classes, tau, kind):
+    """4000 rows in one sequence. A row's error is a few roundings of 2^-24 and averages out (3e-7 a row makes 2e-5 of the
+    sum, five times that is allowed), but for the part that has one sign in all of them: 5e-8 a row is allowed."""
+    rows = 4000
+    x, g = _logits(rows, classes, 0, kind, scale=1.0)
+    labels = torch.randint(0, classes, (rows,), generator=g, device="cuda").int()
+    at = torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda")
+    t = float(np.float32(tau))
+    want = sum(float(torch.log_softmax(a.double() / t, 1).gather(1, b[:, None].long()).sum())
+               for a, b in zip(x.data.split(500), labels.split(500)))
+    ref = torch.tensor([want, 0.0], device="cuda")          # in f32: what it lacks is the margin's
+    got = losses.preference_loss(gpu_ctx, x, labels, at, sk.PreferenceLossConfig(beta=1.0, temperature=tau), logp_ref=ref, gradient=False)
+    assert abs(float(got.margin) - (want - float(ref[0].double()))) <= rows * 5e-8 + 5 * 3e-7 * rows ** 0.5
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [8, 64, 1000])
+def test_labels_that_are_nearly_certain(gpu_ctx, classes, kind):
+    """log p = -log1p(the rest's sum) keeps relative places where the label's own thread adds few classes: at most 4 chains
+    of 8 sums with 1 in them (one unit of it up to 64 classes), 2^-24 each, beside the f32 terms of the rest and the label's own rounding of the difference."""
+    rows = 256
+    for rest in (0.3, 1e-2, 1e-4):
+        x, g = _logits(rows, classes, 0, kind, seed=5, scale=2.0)
+        labels = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+        x.data.scatter_(1, labels[:, None], -INF)
+        top = torch.logsumexp(x.data.float(), 1, keepdim=True) - math.log(rest)
+        x.data.scatter_(1, labels[:, None], top.to(x.data.dtype))
+        want = torch.log_softmax(x.data.double(), 1).gather(1, labels[:, None])[:, 0]
+        got = losses.label_logprob(gpu_ctx, x, labels.int()).logp.double()
+        adds = 6 if classes <= 64 else 32
+        assert ((got - want).abs() <= adds * 2.0 ** -24 + want.abs() * (2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23 * 32)).all()
+
+
 def _calls(x, g, classes):
     rows = x.data.shape[0]
     labels = torch.randint(0, classes, (rows,), generator=g, device="cuda").int()
@@ -696,6 +731,51 @@ def test_losses_without_gradients(gpu_ctx):
     a, b = (losses.preference_loss(gpu_ctx, x, labels, off, gradient=w) for w in (True, False))
     assert b.d_logits is None and torch.equal(a.loss, b.loss) and torch.equal(a.row_logp, b.row_logp)
     del calls
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,classes", [(300, 40009), (7, 131072), (200, 131075), (40, 3001), (700, 90)])
+def test_gradients_over_the_logits_they_come_from(gpu_ctx, rows, classes, kind):
+    """Blocks that share a row write their part while others may still be at theirs."""
+    x, g = _logits(rows, classes, 3, kind, 1, scale=2.0)
+    labels = _label_rows(rows, classes, g)
+    vec = [torch.randn(rows, generator=g, device="cuda") for _ in range(3)]
+    idx, values = _teacher(rows, classes, 40, g)
+    offsets = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device="cuda")
+    cfg = sk.PolicyLossConfig(kl_coeff=0.1, entropy_coeff=0.02)
+    for call in (lambda t, o: losses.label_logprob_backward(gpu_ctx, t, labels, vec[0], vec[1], classes=classes, out=o),
+                 lambda t, o: losses.policy_loss(gpu_ctx, t, labels, vec[0] - 9, vec[1], cfg, logp_ref=vec[2] - 9, classes=classes, out=o).d_logits,
+                 lambda t, o: losses.distill_loss(gpu_ctx, t, idx, values, teacher_lse=vec[0].abs() + 8.0, classes=classes, out=o).d_logits,
+                 lambda t, o: losses.preference_loss(gpu_ctx, t, labels, offsets, classes=classes, out=o).d_logits):
+        want = call(x, None).data
+        flat = torch.empty(x.len() + 1, dtype=x.data.dtype, device="cuda")        # at the same offset within 16 bytes, on which sums depend
+        over = sk.Tensor(flat[1:].view(x.data.shape).copy_(x.data), x.precision, take_id=False)
+        assert call(over, over) is over
+        gpu_ctx.synchronize()
+        assert torch.equal(over.data, want)
+
+
+def test_inputs_of_another_stream_are_kept(gpu_ctx):
+    """A context on a stream of its own: memory of inputs that are dropped right after the call is not handed out while
+    the call still reads it."""
+    side = torch.cuda.Stream()
+    ctx = sk.GpuContext(16, 0, stream=side)
+    rows, classes = 512, 32768
+    x, g = _logits(rows, classes, 0, "bf16")
+    labels = torch.randint(0, classes, (rows,), generator=g, device="cuda").int()
+    want = losses.label_logprob_backward(gpu_ctx, x, labels, torch.full((rows,), 2.0, device="cuda")).data.clone()
+    out = sk.Tensor(torch.empty_like(x.data), sk.Precision.BF16, take_id=False)
+    for _ in range(5):
+        scale = torch.full((rows,), 2.0, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(8):                     # several passes queue up
+            losses.label_logprob_backward(ctx, x, labels, scale, out=out)
+        del scale
+        for _ in range(4):
+            torch.full((rows,), 7.0, device="cuda")
+        ctx.synchronize()
+        assert torch.equal(out.data, want)
+    ctx.close()
 
 
 # ---- networks ----------------------------------------------------------------------------------------------------
