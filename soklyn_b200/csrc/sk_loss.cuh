@@ -222,7 +222,7 @@ template <typename T, int U, int SUMS> __device__ __forceinline__ void accumulat
         if (a.m != -INFINITY) {
             const float d = factor_log<SUMS>(a.m, mx, c_hi, c_lo), f = ex2(d);
             if (SUMS) a.u = moved_u<SUMS>(a.u, a.s, d, f);
-            a.s *= fmaf(f, kEx2Low, f);
+            a.s *= f;                       // lifted with the rest at the end; by itself as well, it would be 2e-8 too much
         }
         a.m = mx;
     }
@@ -314,18 +314,10 @@ template <int NT> struct Team {
     Shared &sh;
     uint32_t tid, lane, rank, ranks, merged, met;
     __device__ __forceinline__ explicit Team(Shared &s) : sh(s), tid(threadIdx.x), lane(threadIdx.x & 31), rank(tc::cluster_rank()), ranks(tc::cluster_size()), merged(0), met(0) {
-        if (ranks > 1) cluster_arrive();
+        if (ranks > 1) tc::cluster_sync<false>();
     }
     // Every team that was set up either meets or leaves.
-    __device__ __forceinline__ void leave() { if (ranks > 1 && met == 0) cluster_wait(); }
-    static __device__ __forceinline__ void cluster_arrive() {
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    }
-    static __device__ __forceinline__ void cluster_wait() {
-        __syncwarp();
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    __device__ __forceinline__ void leave() { if (ranks > 1 && met == 0) tc::cluster_wait(); }
     // The block's statistics from those of its threads, in every thread, in a fixed order. Every warp joins all the
     // warps' parts, a lane to each: one after the other they took 10 % of a row of 64 KB.
     template <int SUMS> __device__ __forceinline__ Stat merge(const Share &share, float c_hi, float c_lo) {
@@ -338,7 +330,7 @@ template <int NT> struct Team {
     // The cluster's from those of its blocks, in a fixed order. All blocks of the cluster, the same number of times.
     template <int SUMS> __device__ __forceinline__ Stat meet(const Stat &a, int flag, float c_hi, float c_lo, int *any) {
         if (ranks == 1) { *any = flag; return a; }
-        if (met == 0) cluster_wait();                    // every block runs: its shared memory may be written
+        if (met == 0) tc::cluster_wait();                    // every block runs: its shared memory may be written
         Message(&box)[kMaxCluster] = sh.box[met++ & 1];  // of the other one a block may still be reading
         if (tid < ranks) {
             const uint32_t at = tc::map_shared(tc::smem_u32(&box[rank]), tid);

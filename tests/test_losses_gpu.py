@@ -701,7 +701,11 @@ def test_rows_behind_32_bits(gpu_ctx):
     ones = torch.ones(rows, device="cuda")
     want = losses.label_logprob_backward(gpu_ctx, tail, labels[-2:].clone(), ones[:2])
     got = losses.label_logprob_backward(gpu_ctx, x, labels, ones, out=x)
-    assert torch.equal(got.data[-2:], want.data)
+    # The two calls share their rows among different numbers of blocks, so the sums are added in another order: chains of
+    # at most 131072 / 1024 + 40 terms of 2^-24 each, below 2^-16 of the sum. Two values that near round to the same f16
+    # or to neighbours, which are at most 2^-10 of the value (2^-24 where it is subnormal) apart.
+    a, b = got.data[-2:].double(), want.data.double()
+    assert ((a - b).abs() <= (b.abs() * 2.0 ** -10).clamp(min=2.0 ** -24) + 2.0 ** -16 * b.abs()).all()
     assert float(got.data[:64].abs().max()) == 0.0 and float(got.data[32800:-2].abs().max()) == 0.0
     del got, x
     torch.cuda.empty_cache()
