@@ -54,7 +54,7 @@ __device__ __forceinline__ double log_wide(float s) {
 // What ex2 lacks: its results are 5.1e-8 too small on average (measured over [-32, 0), weighted by size, the same in every
 // octave; 1.4e-7 at most), and exact for the exponent 0 of a thread's own maximum. It is the same sign in every row, which
 // the sum over a sequence does not average out: it made 8e-6 of a preference margin of sequences that differ by hundreds
-// of rows. A thread's sum is lifted by it.
+// of rows. A thread's sum is lifted by it; what is left is below 1.7e-8 of a sum (4000 rows of 20 to 20000 classes).
 constexpr float kEx2Low = 5.0e-8f;
 
 // The largest of a warp's values, in every lane; one instruction on sm_100a. NaN only if all are.
@@ -194,7 +194,7 @@ struct Stat {
 // -inf makes NaN of e t2 = 0 * -inf; such a row is taken again with kMasked, which bounds t2 at -200, where e is 0 already.
 enum Sums : int { kSums = 0, kEntropy = 1, kMasked = 2 };
 // 2^t for t <= 0, from its power series in the fraction: right to a rounding of either sign. With ex2 for the factors of
-// partial sums, even lifted, up to 1.1e-7 of a row's sum was left; with this 3e-8.
+// partial sums, even lifted, up to 1.1e-7 of a row's sum was left; with this 1.7e-8.
 __device__ __forceinline__ float pow2(float t) {
     if (t < -126.0f) return 0.0f;
     const float n = rintf(t), r = (t - n) * kLn2, r2 = r * r;
