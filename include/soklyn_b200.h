@@ -221,7 +221,8 @@ int sk_output_error(sk_ctx *ctx, const sk_dense *layer, const void *target, uint
  * gradients of zero, whatever they hold; a class at -inf has probability 0; a NaN or +inf makes NaN of its own row.
  * A label or class index at or above `classes` is treated as one below 0 and reported by the next sk_sync
  * (SK_ERR_INDEX_RANGE). Sums and statistics are f32, sums over a sequence f64. rows = 0 is a call without work. Nothing
- * is kept between calls and the context's workspace is not used. Results repeat bit for bit. */
+ * is kept between calls and the context's workspace is not used. The outputs other than d_logits must not overlap an
+ * input. Results of the same sizes at addresses that are equal modulo 16 repeat bit for bit. */
 typedef struct {
     uint32_t dtype;                 /* SK_F32 / SK_F16 / SK_BF16: logits and d_logits */
     uint32_t rows, cols, classes;
