@@ -109,9 +109,14 @@ template <typename T> cudaError_t sequence_gradient_impl(sk_ctx *c, const loss::
     return launch_step(c->stream, overlaps(c), dim3(r.rows), threads, 0, dim3(1), kernel, r, labels, kept);
 }
 template <typename T> cudaError_t distill_impl(sk_ctx *c, const loss::Rows &r, const loss::Distill &op) {
-    const RowPlan plan = plan_row(c, r, sizeof(T), r.d != nullptr);
-    const size_t units = (size_t)r.classes * sizeof(T) / 16, bytes = ((units + plan.ranks - 1) / plan.ranks + 2) * (16 / sizeof(T)) / 8 + 4;   // a bit per class of a part, its edges in units of their own
+    RowPlan plan = plan_row(c, r, sizeof(T), r.d != nullptr);
     const uint32_t threads = std::max(plan.threads, 64u);
+    // A block has 48 KB without asking for more, and a row's bits may take 128: more blocks share such a row (four at 2^20 classes)
+    // rather than one block keeping an SM to itself. A gradient's rows are shared by enough blocks for other reasons.
+    constexpr size_t room = 48 * 1024 - sizeof(loss::DistillShared<kMostThreads>);
+    while (plan.ranks < loss::kMaxCluster && loss::bit_bytes<T>(r.classes, plan.ranks) > room) plan.ranks *= 2;
+    static_assert(loss::kMaxListClasses / loss::kMaxCluster / 8 + 64 <= room, "the bits of the widest row fit the blocks of a cluster");
+    const size_t bytes = loss::bit_bytes<T>(r.classes, plan.ranks);
     auto kernel = threads == 64 ? loss::distill_kernel<T, 64> : threads == 128 ? loss::distill_kernel<T, 128> : loss::distill_kernel<T, kMostThreads>;
     c->launches++;
     c->loss_launches++;

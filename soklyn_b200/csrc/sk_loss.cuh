@@ -792,15 +792,26 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
 // S is a sum of its own over the classes outside (1 - sum p_k would cancel): a bit for each class of the block's part says
 // which are listed, and these count as -inf where the row is summed; they are written by themselves behind the rest of the
 // gradient. Setting its bit also tells an entry whether its class was given before; the masses then add at the class.
+template <int NT> struct DistillShared {
+    typename Team<NT>::Shared team;
+    int32_t idx[kMaxList];
+    struct { float m, to_mass, f, total, of_s, outside; bool dead; } found;   // what the list's warp made of it
+    float val[kMaxList], sx[kMaxList], share[kMaxList];      // the teacher's logit, the student's, the teacher's share (not normalised)
+};
+// Bytes of the bits of one of `ranks` parts of a row: one per class, the head and the tail in units of their own.
+template <typename T> inline size_t bit_bytes(uint32_t classes, uint32_t ranks) {
+    const size_t units = (size_t)classes / Unit<T>::V, words = (((units + ranks - 1) / ranks + 2) * Unit<T>::V + 31) / 32;
+    return words * 4;
+}
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill t) {
     constexpr uint32_t V = Unit<T>::V;
     extern __shared__ uint32_t bits[];
-    __shared__ typename Team<NT>::Shared shared;
-    __shared__ int32_t idx[kMaxList];
-    __shared__ struct { float m, to_mass, f, total, of_s, outside; bool dead; } found;   // what the list's warp made of it
-    __shared__ float val[kMaxList], sx[kMaxList], share[kMaxList];      // the teacher's logit, the student's, the teacher's share (not normalised)
-    Team<NT> team(shared);
+    __shared__ DistillShared<NT> sh;
+    auto &idx = sh.idx;
+    auto &found = sh.found;
+    auto &val = sh.val, &sx = sh.sx, &share = sh.share;
+    Team<NT> team(sh.team);
     const uint32_t row = blockIdx.x / team.ranks, tid = team.tid, lane = team.lane;
     const bool first = tid == 0 && team.rank == 0;
     grid_ready();
