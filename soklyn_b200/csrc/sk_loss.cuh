@@ -795,8 +795,9 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
 template <int NT> struct DistillShared {
     typename Team<NT>::Shared team;
     int32_t idx[kMaxList];
-    struct { float m, to_mass, f, total, of_s, outside; bool dead; } found;   // what the list's warp made of it
-    float val[kMaxList], sx[kMaxList], share[kMaxList];      // the teacher's logit, the student's, the teacher's share (not normalised)
+    struct { double to_mass; float m, f, of_s, outside; bool dead; } found;   // what the list's warp made of it
+    double share[kMaxList];                 // the teacher's share (not normalised): the mass outside the list is 1 less their sum
+    float val[kMaxList], sx[kMaxList];      // the teacher's logit, the student's
 };
 // Bytes of the bits of one of `ranks` parts of a row: one per class, the head and the tail in units of their own.
 template <typename T> inline size_t bit_bytes(uint32_t classes, uint32_t ranks) {
@@ -810,7 +811,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
     __shared__ DistillShared<NT> sh;
     auto &idx = sh.idx;
     auto &found = sh.found;
-    auto &val = sh.val, &sx = sh.sx, &share = sh.share;
+    auto &share = sh.share;
+    auto &val = sh.val, &sx = sh.sx;
     Team<NT> team(sh.team);
     const uint32_t row = blockIdx.x / team.ranks, tid = team.tid, lane = team.lane;
     const bool first = tid == 0 && team.rank == 0;
@@ -848,7 +850,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             const uint32_t b = part.place((uint32_t)idx[i]);
             twice |= (atomicOr(&bits[b / 32], 1u << (b % 32)) >> (b % 32)) & 1u;
         }
-        share[i] = val[i] == -INFINITY ? 0.0f : expf((float)((double)val[i] * r.inv_t - shift));
+        share[i] = val[i] == -INFINITY ? 0.0 : exp((double)val[i] * r.inv_t - shift);
     }
     twice = __syncthreads_or(twice);
     Stat a = team.template merge<kSums>(team.template scan<T, kSums>(x, part, r.c_hi, r.c_lo, [&](Unit<T> &q, uint32_t place) {
@@ -876,12 +878,13 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
         for (uint32_t i = lane; i < t.k; i += 32) {
             const float d = sx[i] - m, e = pow2(fmaf(d, r.c_hi, d * r.c_lo));
             if (leads(i)) listed += e;
-            mass += (double)share[i];
+            mass += share[i];
         }
         listed = warp_sum(listed);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
-        const float s = outside + listed, to_mass = t.lse ? 1.0f : 1.0f / (float)mass;
+        const float s = outside + listed;
+        const double to_mass = t.lse ? 1.0 : (double)(1.0f / (float)mass);
         double rest = t.lse ? 1.0 - mass : 0.0;
         if (rest <= kLeastTail) rest = 0.0;
         if (team.rank == 0 && !dead) {
@@ -889,8 +892,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             double l = 0.0;
             for (uint32_t i = lane; i < t.k; i += 32) {
                 const double log_q = (double)val[i] * r.inv_t - shift - log_mass;
-                const float q = share[i] * to_mass;
-                if (q != 0.0f) l += (double)q * (log_q - (((double)sx[i] - (double)m) * r.inv_t - log_s));
+                const double q = share[i] * to_mass;
+                if (q != 0.0) l += q * (log_q - (((double)sx[i] - (double)m) * r.inv_t - log_s));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -902,9 +905,9 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             found.m = m;
             found.to_mass = to_mass;
             found.f = (float)((double)w * (double)r.k * t.factor);
-            found.total = t.lse ? (float)(mass + rest) : 1.0f;
-            found.of_s = found.total / s;
-            found.outside = outside > 0.0f ? found.of_s - (float)rest / outside : 0.0f;
+            const double total = t.lse ? mass + rest : 1.0;
+            found.of_s = (float)total / s;
+            found.outside = outside > 0.0f ? (float)(total * (double)(outside / s) - rest) / outside : 0.0f;
             found.dead = dead;
         }
     }
@@ -920,11 +923,11 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
     for (uint32_t i = tid; i < t.k; i += NT) {
         if (!mine(i) || !leads(i)) continue;
-        float q = 0.0f;
+        double q = 0.0;
         for (uint32_t o = i; o < (twice ? t.k : i + 1); ++o)
             if (idx[o] == idx[i]) q += share[o] * found.to_mass;
         const float df = sx[i] - found.m, e = ex2(fmaf(df, r.c_hi, df * r.c_lo));
-        d[idx[i]] = from_f32<T>(found.f * (found.of_s * e - q));
+        d[idx[i]] = from_f32<T>(found.f * (found.of_s * e - (float)q));
     }
 }
 

@@ -30,3 +30,53 @@ def test_distillation_without_a_gradient_takes_every_width(gpu_ctx, rows, classe
         s = slice(a, a + 20)
         each, tol, *_ = distill_reference(x.data[s], classes, 1.0, idx[s], values[s], lse[s], None, 1.0)
         _close(got.loss[s], each, tol, "loss")
+
+
+def _tail_reference(x, classes, tau, idx, values, lse, scale):
+    """Loss and gradient of a distillation with its tail, in 64 bits and in logarithms: classes however far below the listed
+    ones count. Tolerances: the list's and the tail's masses are 64 bits and add a rounding to f32; the rest is the two sums."""
+    at = idx.long()
+    logq = values.double() / tau - lse.double()[:, None]
+    q = logq.exp()
+    rest = 1.0 - q.sum(1)
+    assert (rest > 1e-6).all()
+    inside = torch.zeros(x.shape[0], classes, dtype=torch.bool, device=x.device).scatter_(1, at, True)
+    z = x[:, :classes].double() / tau
+    others = torch.where(inside, -INF, x[:, :classes])
+    r, o = Ref(x, classes, tau), Ref(others, classes, tau)
+    log_out = o.lse + (others.double() / tau).amax(1) - r.lse - z.amax(1)
+    loss = (q * (logq - r.lp.gather(1, at))).sum(1) + rest * (rest.log() - log_out)
+    tol = q.sum(1) * r.sum_rel + rest * (r.sum_rel + o.sum_rel) + 2.0 ** -23 * loss.abs()
+    target = torch.zeros_like(r.p).scatter_add_(1, at, q)
+    total, back, f = (q.sum(1) + rest)[:, None], rest[:, None] * o.p, tau * scale
+    want = f * (total * r.p - back - target)
+    tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 0.0, torch.float32: 0.0}[x.dtype]
+    d_tol = (torch.finfo(x.dtype).eps / 2 * want.abs() * (1 + 2.0 ** -10) + tiny
+             + f * ((r.rel + torch.where(inside, 0.0, o.rel)) * total * r.p + o.rel * back + 2.0 ** -22 * target + 1e-36))
+    return loss * tau * tau, tol * tau * tau, want, d_tol
+
+
+def check_tail(ctx, x, classes, tau, idx, values, lse, scale, **kw):
+    loss, tol, want, d_tol = _tail_reference(x.data, classes, tau, idx, values, lse, scale)
+    got = losses.distill_loss(ctx, x, idx, values, sk.DistillLossConfig(tau), teacher_lse=lse, classes=classes, grad_scale=scale, **kw)
+    ctx.synchronize()
+    _close(got.loss, loss, tol, "loss")
+    _close(got.d_logits.data[:, :classes], want, d_tol, "gradient")
+    alone = losses.distill_loss(ctx, x, idx, values, sk.DistillLossConfig(tau), teacher_lse=lse, classes=classes, gradient=False)
+    _close(alone.loss, loss, tol, "loss without a gradient")
+
+
+def _with_tail(values, tau, tail):
+    return (torch.logsumexp(values.double() / tau, 1) - math.log1p(-tail)).float()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("classes,k", [(13, 12), (1000, 64), (40009, 300), (131072, 512)])
+def test_a_small_tail_keeps_its_places(gpu_ctx, classes, k, kind):
+    """1 minus the sum of the list's masses: with those in f32 a tail of 1e-5 would be off by a hundredth, and with it the
+    gradient of every class outside the list."""
+    for tail in (0.2, 1e-3, 1e-5):
+        x, g = _logits(40, classes, 3, kind, 1, scale=1.0)
+        idx, values = _teacher(40, classes, k, g)
+        lse = _with_tail(values, 1.0, tail)
+        check_tail(gpu_ctx, x, classes, 1.0, idx, values, lse, 1.0)
