@@ -792,10 +792,12 @@ __device__ __forceinline__ float teacher_value(const Distill &d, size_t i) {
 // S is a sum of its own over the classes outside (1 - sum p_k would cancel): a bit for each class of the block's part says
 // which are listed, and these count as -inf where the row is summed; they are written by themselves behind the rest of the
 // gradient. Setting its bit also tells an entry whether its class was given before; the masses then add at the class.
+// The classes outside keep their own maximum: relative to the row's they vanish where the student holds the list 87 (in
+// (x - m) / T) or more above them, and with them log S and the term r e_j / (sum of e outside), whose sum is r all the same.
 template <int NT> struct DistillShared {
     typename Team<NT>::Shared team;
     int32_t idx[kMaxList];
-    struct { double to_mass; float m, f, of_s, outside; bool dead; } found;   // what the list's warp made of it
+    struct { double to_mass; float m, m_out, f, of_s, outside; bool dead; } found;   // what the list's warp made of it
     double share[kMaxList];                 // the teacher's share (not normalised): the mass outside the list is 1 less their sum
     float val[kMaxList], sx[kMaxList];      // the teacher's logit, the student's
 };
@@ -897,7 +899,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (rest > 0.0) l += rest * (log(rest) - (outside > 0.0f ? log_wide(outside) - log_s : -INFINITY));
+            if (rest > 0.0) l += rest * (log(rest) - (a.m == -INFINITY ? (a.more == 0.0f ? -INFINITY : (double)a.more) : ((double)a.m - (double)m) * r.inv_t + a.log_s() - log_s));
             if (first) t.loss[row] = (float)(t.factor * (double)w * l);
         }
         if (tid == 0) {
@@ -907,7 +909,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             found.f = (float)((double)w * (double)r.k * t.factor);
             const double total = t.lse ? mass + rest : 1.0;
             found.of_s = (float)total / s;
-            found.outside = outside > 0.0f ? (float)(total * (double)(outside / s) - rest) / outside : 0.0f;
+            found.m_out = a.m == -INFINITY ? 0.0f : a.m;
+            found.outside = a.m == -INFINITY ? 0.0f : (float)(total * (double)(outside / s) - rest) / a.s();
             found.dead = dead;
         }
     }
@@ -918,7 +921,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
     __syncthreads();
     if (found.dead) return nothing_to_learn();
     if (!r.d) return;
-    write_row<T, NT, kSums>(r, row, part, team.rank, team.ranks, found.m, Coef{found.f * found.outside, 0.0f, 0.0f}, -1, 0.0f);
+    write_row<T, NT, kSums>(r, row, part, team.rank, team.ranks, found.m_out, Coef{found.f * found.outside, 0.0f, 0.0f}, -1, 0.0f);
     __syncthreads();                        // the list's classes are written again, with their own values
     T *d = reinterpret_cast<T *>(r.d) + (size_t)row * r.cols;
     for (uint32_t i = tid; i < t.k; i += NT) {

@@ -80,3 +80,16 @@ def test_a_small_tail_keeps_its_places(gpu_ctx, classes, k, kind):
         idx, values = _teacher(40, classes, k, g)
         lse = _with_tail(values, 1.0, tail)
         check_tail(gpu_ctx, x, classes, 1.0, idx, values, lse, 1.0)
+
+
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes,pad,offset", [(10, 3, 1), (1000, 0, 0), (5003, 0, 2), (70001, 7, 1)])
+def test_a_tail_far_below_the_listed_classes(gpu_ctx, classes, pad, offset, kind):
+    """The student's mass outside the list from e^-40 to far below what f32 holds: the loss grows with its logarithm and the
+    gradient still moves the tail's whole mass to the classes outside."""
+    for tau in (1.0, 0.25, 2.0 ** -6):
+        for gap, tail in ((40.0, 0.2), (86.0, 0.2), (87.5, 1e-3), (88.5, 0.2), (104.0, 1e-3), (200.0, 0.2), (4000.0, 0.2)):
+            x, g = _logits(5, classes, pad, kind, offset, scale=3.0 * tau)
+            idx, values = _teacher(5, classes, 4, g, spread=tau)
+            x.data.scatter_add_(1, idx.long(), torch.full((5, 4), gap * tau, device="cuda").to(x.data.dtype))
+            check_tail(gpu_ctx, x, classes, tau, idx, values, _with_tail(values, tau, tail), 32.0)
