@@ -63,6 +63,17 @@ __device__ __forceinline__ float max_of_warp(float v) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
+// The same with NaN as soon as one of them is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_of_warp_or_nan(float v) {
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 
 // ---- 16 bytes of a row, and pairs of f32 values ------------------------------------------------
 // Arithmetic is on pairs (add / mul / fma.rn.f32x2: two round-to-nearest operations in one instruction), because wide
@@ -872,8 +883,9 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
     };
     if (tid < 32) {                         // the list is one warp's
         float best = -INFINITY, listed = 0.0f;
-        for (uint32_t i = lane; i < t.k; i += 32) best = fmaxf(best, sx[i]);
-        const float m = fmaxf(a.m, max_of_warp(best));
+        for (uint32_t i = lane; i < t.k; i += 32) best = max_or_nan(best, sx[i]);
+        // NaN beside classes at -inf alone is no empty row
+        const float m = max_or_nan(a.m == -INFINITY ? a.m + a.more : a.m, max_of_warp_or_nan(best));
         const bool dead = (!t.lse && (!some || top == -INFINITY)) || (m == -INFINITY && a.more == 0.0f);
         const float outside = a.m == -INFINITY ? a.more : a.s() * pow2(factor_log<kSums>(a.m, m, r.c_hi, r.c_lo));
         double mass = 0.0;
@@ -909,7 +921,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_kernel(Rows r, Distill 
             found.f = (float)((double)w * (double)r.k * t.factor);
             const double total = t.lse ? mass + rest : 1.0;
             found.of_s = (float)total / s;
-            found.m_out = a.m == -INFINITY ? 0.0f : a.m;
+            found.m_out = a.m == -INFINITY ? m - m : a.m;      // none: 0, or NaN for the row
             found.outside = a.m == -INFINITY ? 0.0f : (float)(total * (double)(outside / s) - rest) / a.s();
             found.dead = dead;
         }

@@ -93,3 +93,22 @@ def test_a_tail_far_below_the_listed_classes(gpu_ctx, classes, pad, offset, kind
             idx, values = _teacher(5, classes, 4, g, spread=tau)
             x.data.scatter_add_(1, idx.long(), torch.full((5, 4), gap * tau, device="cuda").to(x.data.dtype))
             check_tail(gpu_ctx, x, classes, tau, idx, values, _with_tail(values, tau, tail), 32.0)
+
+
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes", [12, 5003, 70001])
+def test_a_listed_nan_beside_masked_classes_is_not_an_empty_row(gpu_ctx, classes, kind):
+    x, g = _logits(4, classes, 1, kind, 1)
+    idx, values = _teacher(4, classes, 4, g)
+    x.data[:2, :classes] = -INF
+    x.data[0, idx[0, 2].long()] = math.nan
+    kept = x.data[3, idx[3].long()].clone()
+    x.data[3, :classes] = -INF
+    outside = min(set(range(5)) - set(idx[3].tolist()))
+    x.data[3, idx[3].long()], x.data[3, outside] = kept, math.nan      # a class outside is NaN, the others there are masked
+    for lse in (None, _with_tail(values, 1.0, 0.2)):
+        got = losses.distill_loss(gpu_ctx, x, idx, values, teacher_lse=lse, classes=classes)
+        assert got.loss[0].isnan() and got.d_logits.data[0, :classes].isnan().all()
+        assert float(got.loss[1]) == 0.0 and (got.d_logits.data[1] == 0).all()       # no class at all: does not count
+        assert got.loss[2].isfinite() and got.d_logits.data[2].isfinite().all()
+        assert got.loss[3].isnan() and got.d_logits.data[3, :classes].isnan().all()
