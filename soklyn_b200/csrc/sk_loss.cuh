@@ -529,9 +529,12 @@ struct Policy {
         loss[row] = logp[row] = kl[row] = 0.0f;
         if (entropy) entropy[row] = 0.0f;
     }
-    // exp(d) - 1 - d without the cancellation of small d
+    // exp(d) - 1 - d without the cancellation of small d; infinite for an action that is masked (d = inf)
     static __device__ __forceinline__ float expm1_less(float d) {
-        if (fabsf(d) > 0.5f) return expm1f(d) - d;
+        if (fabsf(d) > 0.5f) {
+            const float e = expm1f(d);
+            return e == INFINITY ? e : e - d;
+        }
         float p = 1.0f / 40320.0f;
         p = fmaf(p, d, 1.0f / 5040.0f); p = fmaf(p, d, 1.0f / 720.0f); p = fmaf(p, d, 1.0f / 120.0f);
         p = fmaf(p, d, 1.0f / 24.0f); p = fmaf(p, d, 1.0f / 6.0f); p = fmaf(p, d, 0.5f);
@@ -545,11 +548,11 @@ struct Policy {
         const float plain = rho * adv, held = fminf(fmaxf(rho, lo), hi) * adv;
         const bool clipped = (adv > 0.0f && rho > hi) || (adv < 0.0f && rho < lo);
         float g = clipped ? 0.0f : -plain;
-        if (ref) g -= beta * expm1f(d);
+        if (beta != 0.0f) g -= beta * expm1f(d);      // not 0 * inf: without the factor the KL is reported only
         const float kl_v = ref ? expm1_less(d) : 0.0f;
         if (first) {
             float l = fmaxf(-plain, -held);
-            if (ref) l += beta * kl_v;
+            if (beta != 0.0f) l += beta * kl_v;
             if (eta != 0.0f) l -= eta * h;
             loss[row] = w * l;
             logp[row] = (float)lp;

@@ -112,3 +112,28 @@ def test_a_listed_nan_beside_masked_classes_is_not_an_empty_row(gpu_ctx, classes
         assert float(got.loss[1]) == 0.0 and (got.d_logits.data[1] == 0).all()       # no class at all: does not count
         assert got.loss[2].isfinite() and got.d_logits.data[2].isfinite().all()
         assert got.loss[3].isnan() and got.d_logits.data[3, :classes].isnan().all()
+
+
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes", [10, 5000])
+@pytest.mark.parametrize("eta", [0.0, 0.02])
+def test_a_kl_that_is_only_watched_changes_nothing(gpu_ctx, eta, classes, kind):
+    """kl_coeff = 0 with a reference given: the KL is reported, infinite or not, and is no term of the loss."""
+    x, g = _logits(4, classes, 0, kind)
+    actions = torch.randint(0, classes, (4,), generator=g, device="cuda").int()
+    x.data[0, actions[0].long()] = -INF                    # a masked action
+    r = Ref(x.data, classes, 1.0)
+    lp = r.pick(actions)
+    ref = lp.nan_to_num(neginf=-3.0) + torch.tensor([0.0, 200.0, -200.0, 0.5], device="cuda")
+    ref, old, adv = ref.float(), lp.nan_to_num(neginf=-5.0).float(), torch.tensor([1.0, -1.0, 1.0, -1.0], device="cuda")
+    cfg = sk.PolicyLossConfig(entropy_coeff=eta)
+    want = losses.policy_loss(gpu_ctx, x, actions, old, adv, cfg)
+    got = losses.policy_loss(gpu_ctx, x, actions, old, adv, cfg, logp_ref=ref)
+    for name in ("loss", "logp", "entropy"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
+    assert torch.equal(got.d_logits.data, want.d_logits.data)
+    assert got.loss.isfinite().all() and got.d_logits.data.isfinite().all()
+    d = ref.double() - lp
+    assert float(got.kl[0]) == INF and float(got.kl[1]) == INF       # exp(200) is beyond f32
+    tol = torch.expm1(d).abs() * r.sum_rel + r.sum_rel + 2.0 ** -22 * d.abs()
+    _close(got.kl[2:], (torch.expm1(d) - d)[2:], tol[2:], "kl")
