@@ -545,7 +545,7 @@ struct Policy {
         const float w = in.w, adv = in.adv;
         const float rho = expf((float)(lp - (double)in.old));
         const float d = ref ? (float)((double)in.ref - lp) : 0.0f, h = (float)(log_s - (double)(a.u / a.s() * kLn2));
-        const float plain = rho * adv, held = fminf(fmaxf(rho, lo), hi) * adv;
+        const float plain = adv == 0.0f && rho == INFINITY ? 0.0f : rho * adv, held = fminf(fmaxf(rho, lo), hi) * adv;
         const bool clipped = (adv > 0.0f && rho > hi) || (adv < 0.0f && rho < lo);
         float g = clipped ? 0.0f : -plain;
         if (beta != 0.0f) g -= beta * expm1f(d);      // not 0 * inf: without the factor the KL is reported only

@@ -137,3 +137,17 @@ def test_a_kl_that_is_only_watched_changes_nothing(gpu_ctx, eta, classes, kind):
     assert float(got.kl[0]) == INF and float(got.kl[1]) == INF       # exp(200) is beyond f32
     tol = torch.expm1(d).abs() * r.sum_rel + r.sum_rel + 2.0 ** -22 * d.abs()
     _close(got.kl[2:], (torch.expm1(d) - d)[2:], tol[2:], "kl")
+
+
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes", [10, 5000])
+def test_an_advantage_of_zero_pulls_nowhere(gpu_ctx, classes, kind):
+    """However unlikely the action was: a ratio beyond f32 times no advantage is no loss."""
+    x, g = _logits(3, classes, 0, kind)
+    actions = torch.randint(0, classes, (3,), generator=g, device="cuda").int()
+    old, adv = torch.full((3,), -200.0, device="cuda"), torch.tensor([0.0, -0.0, 0.0], device="cuda")
+    got = losses.policy_loss(gpu_ctx, x, actions, old, adv)
+    assert (got.loss == 0).all() and (got.d_logits.data == 0).all()
+    got = losses.policy_loss(gpu_ctx, x, actions, old, adv, sk.PolicyLossConfig(entropy_coeff=0.5))
+    near = losses.policy_loss(gpu_ctx, x, actions, got.logp, adv, sk.PolicyLossConfig(entropy_coeff=0.5))
+    assert torch.equal(got.loss, near.loss) and torch.equal(got.d_logits.data, near.d_logits.data) and got.d_logits.data.isfinite().all()
