@@ -551,7 +551,7 @@ struct Policy {
         if (beta != 0.0f) g -= beta * expm1f(d);      // not 0 * inf: without the factor the KL is reported only
         const float kl_v = ref ? expm1_less(d) : 0.0f;
         if (first) {
-            float l = fmaxf(-plain, -held);
+            float l = clipped ? -held : -plain;      // the larger one, or NaN, which a maximum would drop
             if (beta != 0.0f) l += beta * kl_v;
             if (eta != 0.0f) l -= eta * h;
             loss[row] = w * l;

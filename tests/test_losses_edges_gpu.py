@@ -151,3 +151,20 @@ def test_an_advantage_of_zero_pulls_nowhere(gpu_ctx, classes, kind):
     got = losses.policy_loss(gpu_ctx, x, actions, old, adv, sk.PolicyLossConfig(entropy_coeff=0.5))
     near = losses.policy_loss(gpu_ctx, x, actions, got.logp, adv, sk.PolicyLossConfig(entropy_coeff=0.5))
     assert torch.equal(got.loss, near.loss) and torch.equal(got.d_logits.data, near.d_logits.data) and got.d_logits.data.isfinite().all()
+
+
+@pytest.mark.parametrize("kind", DT)
+@pytest.mark.parametrize("classes", [10, 5000])
+def test_nan_reaches_the_policy_loss(gpu_ctx, classes, kind):
+    """NaN or +inf among a row's logits, or NaN in its inputs, makes NaN of its loss and gradient on either side of the clip."""
+    x, g = _logits(7, classes, 0, kind)
+    actions = torch.zeros(7, dtype=torch.int32, device="cuda")
+    adv = torch.tensor([1.0, -1.0, 0.0, 1.0, -1.0, math.nan, 1.0], device="cuda")
+    old = torch.full((7,), -3.0, device="cuda")
+    x.data[0:3, 4] = math.nan
+    x.data[3, 5] = INF
+    old[4] = math.nan
+    for eta in (0.0, 0.1):
+        got = losses.policy_loss(gpu_ctx, x, actions, old, adv, sk.PolicyLossConfig(entropy_coeff=eta))
+        assert got.loss[:6].isnan().all() and got.logp[:4].isnan().all() and got.d_logits.data[:6].isnan().all()
+        assert got.loss[6].isfinite() and got.d_logits.data[6].isfinite().all()
