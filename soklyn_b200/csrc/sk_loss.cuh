@@ -746,8 +746,8 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(Pairs p) {
         if (p.smooth > 0.0) value += p.smooth * (l + fmax(m, 0.0));   // not 0 * inf
         slope = p.smooth - 1.0 / (1.0 + exp(m));
     } else if (p.form == SK_PREFERENCE_HINGE) {
-        value = fmax(1.0 - m, 0.0);
-        slope = m < 1.0 ? -1.0 : 0.0;
+        value = m >= 1.0 ? 0.0 : 1.0 - m;                // not fmax, which drops NaN
+        slope = m < 1.0 ? -1.0 : m >= 1.0 ? 0.0 : m;
     } else {
         value = (m - 0.5) * (m - 0.5);
         slope = 2.0 * (m - 0.5);

@@ -168,3 +168,22 @@ def test_nan_reaches_the_policy_loss(gpu_ctx, classes, kind):
         got = losses.policy_loss(gpu_ctx, x, actions, old, adv, sk.PolicyLossConfig(entropy_coeff=eta))
         assert got.loss[:6].isnan().all() and got.logp[:4].isnan().all() and got.d_logits.data[:6].isnan().all()
         assert got.loss[6].isfinite() and got.d_logits.data[6].isfinite().all()
+
+
+@pytest.mark.parametrize("form", sk.PreferenceForm)
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_nan_reaches_the_preference_loss(gpu_ctx, kind, form):
+    """A pair with a NaN in one of its rows has no margin, in any form of the loss; the other pair keeps its results."""
+    x, g = _logits(12, 700, 0, kind)
+    labels = torch.randint(0, 700, (12,), generator=g, device="cuda").int()
+    labels[1] = -1
+    offsets = torch.tensor([0, 3, 6, 9, 12], dtype=torch.int32, device="cuda")
+    cfg = sk.PreferenceLossConfig(form)
+    want = losses.preference_loss(gpu_ctx, x, labels, offsets, cfg)
+    clean = [t.clone() for t in (want.loss[1], want.margin[1], want.d_logits.data[6:])]
+    x.data[4, 9] = math.nan
+    got = losses.preference_loss(gpu_ctx, x, labels, offsets, cfg)
+    assert got.margin[0].isnan() and got.loss[0].isnan() and got.row_logp[4].isnan()
+    counted = [r for r in range(6) if r != 1]
+    assert got.d_logits.data[counted].isnan().all() and (got.d_logits.data[1] == 0).all()
+    assert all(torch.equal(a, b) for a, b in zip((got.loss[1], got.margin[1], got.d_logits.data[6:]), clean))
