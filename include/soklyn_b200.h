@@ -137,7 +137,8 @@ int sk_ctx_set_option(sk_ctx *ctx, uint32_t option, uint32_t value);
 int sk_ctx_reserve(sk_ctx *ctx, size_t workspace_bytes);
 /* CudaStream::synchronize as called after every launch in src/io/device/ffn_device.rs:75,110,136.
  * Also reports SK_ERR_DEVICE_TIMEOUT if a tensor-core kernel abandoned a bounded wait, and SK_ERR_INDEX_RANGE if a loss
- * (sk_label_logprob and what follows it) met an index out of range since the last call. */
+ * (sk_label_logprob and what follows it) met an index out of range since the last call. One report per call: where both
+ * happened, the index is reported by the call after that of the timeout. */
 int sk_sync(sk_ctx *ctx);
 /* Text for a status code, and the detail of the last failure on this context. */
 const char *sk_status_string(int status);

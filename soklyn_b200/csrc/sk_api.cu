@@ -1083,7 +1083,8 @@ int sk_sync(sk_ctx *c) {
     if (rc || !c->tc_err || (c->tc_launches == 0 && c->loss_launches == 0)) return rc;
     int flag[2] = {0, 0};
     if ((rc = check_cuda(c, cudaMemcpy(flag, c->tc_err, sizeof flag, cudaMemcpyDeviceToHost), "error flag read"))) return rc;
-    if (flag[0] != 0 || flag[1] != 0) cudaMemset(c->tc_err, 0, sizeof flag);
+    // one report per call: an index out of range beside a timeout stands until the next one
+    if (flag[0] != 0 || flag[1] != 0) cudaMemset(flag[0] != 0 ? c->tc_err : c->loss_err, 0, sizeof(int));
     if (flag[0] != 0)
         return fail(c, SK_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (code %d: 1 TMA loader, 2 MMA issuer, 3 GEMM epilogue, 5 peer flags)", flag[0]);
     if (flag[1] != 0)

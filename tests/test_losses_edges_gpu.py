@@ -187,3 +187,16 @@ def test_nan_reaches_the_preference_loss(gpu_ctx, kind, form):
     counted = [r for r in range(6) if r != 1]
     assert got.d_logits.data[counted].isnan().all() and (got.d_logits.data[1] == 0).all()
     assert all(torch.equal(a, b) for a, b in zip((got.loss[1], got.margin[1], got.d_logits.data[6:]), clean))
+
+
+def test_an_index_out_of_range_is_reported_beside_a_timeout(gpu_ctx):
+    """A wait that ran out and a label out of range since the last synchronize: one report each."""
+    x, _ = _logits(2, 50, 0, "f32")
+    flags = torch.zeros(4, dtype=torch.int32, device=gpu_ctx.device)
+    losses.label_logprob(gpu_ctx, x, torch.tensor([3, 50], dtype=torch.int32, device="cuda"))
+    gpu_ctx.wait_flags(flags.data_ptr(), 2, 1)              # nobody sets them: gives up after about two seconds
+    with pytest.raises(log.NativeError, match="status 11"):
+        gpu_ctx.synchronize()
+    with pytest.raises(log.IndexOutOfRange, match="a label"):
+        gpu_ctx.synchronize()
+    gpu_ctx.synchronize()
