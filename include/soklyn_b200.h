@@ -169,7 +169,7 @@ int sk_step_abort(sk_ctx *ctx);
 int sk_step_stats(const sk_ctx *ctx, uint64_t out[4]);
 /* A host that allocates device memory while a step is being recorded (cudaMalloc is refused then) brackets the
  * allocation with allow = 1 and allow = 0, on the thread that records. What it allocates has to live until the step has
- * been launched. Does nothing outside a recorded step. */
+ * been launched. allow = 0 puts the thread's capture mode back as allow = 1 found it. Does nothing outside a recorded step. */
 int sk_step_allocations(sk_ctx *ctx, int allow);
 
 /* Per-kernel-class device timing (no counterpart; the reference times phases on the host,

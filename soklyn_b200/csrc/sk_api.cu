@@ -1173,9 +1173,13 @@ int sk_step_stats(const sk_ctx *c, uint64_t out[4]) {
 
 int sk_step_allocations(sk_ctx *c, int allow) {
     if (!c) return SK_ERR_NULL_POINTER;
-    if (!c->step_capturing) return SK_OK;
-    cudaStreamCaptureMode mode = allow ? cudaStreamCaptureModeRelaxed : cudaStreamCaptureModeGlobal;   // a thread's mode is global unless changed
-    return check_cuda(c, cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+    if (allow ? !c->step_capturing || c->allocating : !c->allocating) return SK_OK;
+    cudaStreamCaptureMode mode = allow ? cudaStreamCaptureModeRelaxed : c->caller_mode;
+    const int rc = check_cuda(c, cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+    if (rc) return rc;
+    c->allocating = allow != 0;
+    if (allow) c->caller_mode = mode;   // put back as it was found
+    return SK_OK;
 }
 
 int sk_ctx_set_option(sk_ctx *c, uint32_t option, uint32_t value) {

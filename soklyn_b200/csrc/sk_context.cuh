@@ -57,6 +57,8 @@ struct sk_ctx {
     StepGraph step_graphs[SK_STEP_SLOTS];
     int step_open = -1;                    // slot between begin and end
     bool step_capturing = false;
+    bool allocating = false;               // between sk_step_allocations(1) and (0), with the capture mode the thread had
+    cudaStreamCaptureMode caller_mode = cudaStreamCaptureModeGlobal;
     cudaStream_t record_stream = nullptr;  // the calls of a step are recorded on this stream (the legacy default stream
     cudaStream_t user_stream = nullptr;    // cannot be captured); `stream` points here meanwhile, user_stream keeps the caller's
     uint64_t step_stats[4] = {0, 0, 0, 0}; // instantiated, updated in place, launched, unrecorded steps

@@ -200,3 +200,27 @@ def test_an_index_out_of_range_is_reported_beside_a_timeout(gpu_ctx):
     with pytest.raises(log.IndexOutOfRange, match="a label"):
         gpu_ctx.synchronize()
     gpu_ctx.synchronize()
+
+
+def test_the_threads_capture_mode_is_put_back(gpu_ctx):
+    """Outputs that are allocated while a step is recorded change the thread's capture mode for the allocation alone."""
+    exchange = C.CDLL("libcuda.so.1").cuThreadExchangeStreamCaptureMode
+
+    def swap(mode):
+        m = C.c_int(mode)
+        assert exchange(C.byref(m)) == 0
+        return m.value
+
+    x, _ = _logits(3, 50, 0, "f32")
+    labels = torch.zeros(3, dtype=torch.int32, device="cuda")
+    before = swap(1)                                        # thread-local
+    try:
+        for _ in range(3):                                  # the slot's first step may run unrecorded
+            with gpu_ctx.step_graph(6):
+                losses.label_logprob(gpu_ctx, x, labels)
+                inside = swap(1)
+            gpu_ctx.synchronize()
+            assert inside == 1
+        assert swap(1) == 1
+    finally:
+        swap(before)
