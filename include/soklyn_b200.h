@@ -278,7 +278,8 @@ int sk_policy_loss(sk_ctx *ctx, const sk_logits *logits, const sk_policy *policy
  *   HINGE    loss = w max(0, 1 - margin)
  *   SQUARED  loss = w (margin - 1/2)^2
  * Rows below offsets[0] and from offsets[2 pairs] on belong to no sequence: log-probability and gradient zero. Offsets
- * that fall, or leave [0, rows], make their sequence an empty one and are reported by the next sk_sync. */
+ * that fall, or leave [0, rows], make their sequence an empty one and are reported by the next sk_sync; rows that then
+ * belong to sequences of several pairs get the sum of their gradients. */
 typedef struct {
     const int32_t *labels;          /* [rows] */
     const int32_t *offsets;         /* [2 pairs + 1] */

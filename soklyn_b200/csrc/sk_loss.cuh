@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(kThreads) pair_kernel(Pairs p) {
         double g = w * slope * (h ? -p.beta : p.beta);
         if (p.average && n[h]) g /= (double)n[h];
         for (int32_t r = from[h] + (int32_t)threadIdx.x; r < to[h]; r += kThreads)
-            if (p.kept[r].s != 0.0f) p.kept[r].g = (float)g;
+            if (p.kept[r].s != 0.0f) atomicAdd(&p.kept[r].g, (float)g);      // 0 before: its pair's alone, unless offsets fall and pairs overlap
     }
 }
 

@@ -224,3 +224,35 @@ def test_the_threads_capture_mode_is_put_back(gpu_ctx):
         assert swap(1) == 1
     finally:
         swap(before)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_offsets_that_fall_give_shared_rows_both_gradients(gpu_ctx, kind):
+    """Offsets that fall leave an empty sequence, and the next one may begin inside the one before it: a row of two pairs
+    gets the gradient of both losses, in every run."""
+    rows, classes = 600, 40
+    x, g = _logits(rows, classes, 0, kind)
+    labels = torch.randint(0, classes, (rows,), generator=g, device="cuda").int()
+    cuts = [0, 400, 200, 500, 600]                          # pair 0: [0, 400) and none; pair 1: [200, 500) and [500, 600)
+    ref = torch.tensor([-900.0, 0.0, -700.0, -250.0], device="cuda")
+    beta = 2.0 ** -7
+    r = Ref(x.data, classes, 1.0)
+    lp = r.pick(labels)
+    pull = torch.zeros(rows, dtype=torch.float64, device="cuda")
+    off = torch.zeros(rows, dtype=torch.float64, device="cuda")
+    for chosen, rejected, i in ((slice(0, 400), slice(0, 0), 0), (slice(200, 500), slice(500, 600), 2)):
+        m = beta * (lp[chosen].sum() - ref[i].double() - lp[rejected].sum() + ref[i + 1].double())
+        slope, m_tol = -torch.sigmoid(-m) * beta, beta * (r.sum_rel[chosen].sum() + r.sum_rel[rejected].sum())
+        pull[chosen] += slope
+        pull[rejected] -= slope
+        off[chosen] += 0.25 * beta * m_tol
+        off[rejected] += 0.25 * beta * m_tol
+    hit = torch.zeros_like(r.p).scatter_(1, labels.long()[:, None], 1.0)
+    want, size = pull[:, None] * (hit - r.p), pull.abs()[:, None] * (hit + r.p)
+    tiny = 2.0 ** -25 if kind == "f16" else 0.0
+    tol = torch.finfo(x.data.dtype).eps / 2 * want.abs() * (1 + 2.0 ** -10) + (r.rel + 2.0 ** -22) * size + off[:, None] * (hit + r.p) + tiny
+    for _ in range(4):
+        got = losses.preference_loss(gpu_ctx, x, labels, torch.tensor(cuts, dtype=torch.int32, device="cuda"), sk.PreferenceLossConfig(beta=beta), logp_ref=ref)
+        with pytest.raises(log.IndexOutOfRange, match="offset"):
+            gpu_ctx.synchronize()
+        _close(got.d_logits.data, want, tol, "gradient")
