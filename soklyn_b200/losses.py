@@ -91,6 +91,13 @@ _POLICY = struct.Struct("@PPPPPffffPPPP")
 _PREFERENCE = struct.Struct("@PPIIIPPfffPPPPP")
 
 
+_MAX_F32 = torch.finfo(torch.float32).max
+
+
+def _in_f32(v: float) -> bool:
+    return abs(v) <= _MAX_F32               # finite in the descriptors, too
+
+
 class _Call:
     """Checked logits of one call, the tensors it reads, and its outputs, allocated on the context's stream."""
 
@@ -112,7 +119,7 @@ class _Call:
             raise log.AllocationLimitExceeded(max(rows, cols), 1 << 30, "rows or columns of logits")
         if not 1e-4 <= temperature <= 1e4:
             raise log.InvalidConfiguration(f"Temperature {temperature} must lie between 1e-4 and 1e4.")
-        if not math.isfinite(grad_scale):
+        if not _in_f32(grad_scale):
             raise log.InvalidConfiguration("The gradient scale must be finite.")
         self.data, self.precision, self.classes, self.temperature, self.grad_scale = data, logits.precision, classes, temperature, grad_scale
         self.used = []
@@ -229,9 +236,9 @@ def policy_loss(context, logits: Tensor, actions: torch.Tensor, logp_old, advant
     """Clipped policy loss of each row's action, with a KL term to a reference policy and an entropy bonus."""
     call = _Call(context, logits, classes, config.temperature, grad_scale)
     low, high, beta, eta = config.clip_low, config.clip_high, config.kl_coeff, config.entropy_coeff
-    if not (0.0 <= low <= 1.0 and high >= 0.0):
+    if not (0.0 <= low <= 1.0 and (0.0 <= high <= _MAX_F32 or high == math.inf)):
         raise log.InvalidConfiguration(f"Clip range {low} below and {high} above 1.")
-    if not (math.isfinite(beta) and math.isfinite(eta)):
+    if not (_in_f32(beta) and _in_f32(eta)):
         raise log.InvalidConfiguration("Policy coefficients must be finite.")
     if beta != 0.0 and logp_ref is None:
         raise log.InvalidConfiguration("A KL term needs the reference's log-probabilities.")
@@ -255,7 +262,7 @@ def preference_loss(context, logits: Tensor, labels: torch.Tensor, offsets: torc
     """Preference loss over pairs of packed sequences: rows [offsets[s], offsets[s + 1]) are sequence s, of which 2i is the
     preferred one of pair i and 2i + 1 the other; `logp_ref` [2 pairs] holds the reference's sums (or means)."""
     call = _Call(context, logits, classes, config.temperature, grad_scale)
-    if not (math.isfinite(config.beta) and math.isfinite(config.target_margin)):
+    if not (_in_f32(config.beta) and _in_f32(config.target_margin)):
         raise log.InvalidConfiguration("Beta and target margin must be finite.")
     if not 0.0 <= config.label_smoothing <= 1.0:
         raise log.InvalidConfiguration(f"Label smoothing {config.label_smoothing} must lie between 0 and 1.")
