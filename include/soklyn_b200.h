@@ -219,7 +219,8 @@ int sk_output_error(sk_ctx *ctx, const sk_dense *layer, const void *target, uint
  * an element is taken; rows whose pitch is no multiple of 16 bytes cost a little more, and a gradient that does not lie
  * on the same offset within 16 bytes as its logits is stored element by element.
  * Rows that do not count (a label below 0, a weight of 0, no class above -inf) get losses, log-probabilities and
- * gradients of zero, whatever they hold; a class at -inf has probability 0; a NaN or +inf makes NaN of its own row.
+ * gradients of zero, whatever they hold; a class at -inf has probability 0; a NaN or +inf makes NaN of its own row (and
+ * of the pair it belongs to). A pair whose weight is 0 has a loss and gradients of zero; its margin and log-probabilities are still written.
  * A label or class index at or above `classes` is treated as one below 0 and reported by the next sk_sync
  * (SK_ERR_INDEX_RANGE). Sums and statistics are f32, sums over a sequence f64. rows = 0 is a call without work. Nothing
  * is kept between calls and the context's workspace is not used. The outputs other than d_logits must not overlap an
@@ -242,7 +243,8 @@ int sk_label_logprob_backward(sk_ctx *ctx, const sk_logits *logits, const int32_
                               const float *d_entropy);
 
 /* Distillation from a teacher's top logits: k (class, logit) pairs per row, in any order; entries with an index below 0
- * are unused, an index given twice adds up at its class. Without `lse` the teacher's distribution q is the softmax of
+ * are unused. An index given twice stands for two entries, each with a term of its own in the loss; in the gradient their
+ * masses add up at the class. Without `lse` the teacher's distribution q is the softmax of
  * values / temperature over the list and loss = w T^2 sum q (log q - log p). With `lse` (log-sum-exp of the teacher's
  * logits / temperature over ALL its classes) q = exp(values / temperature - lse), and the mass r = 1 - sum q outside the
  * list, where it is above 1e-6, is compared with the student's mass outside it: + r (log r - log S). A row with an empty
@@ -259,7 +261,8 @@ int sk_distill_loss(sk_ctx *ctx, const sk_logits *logits, const sk_distill *teac
 /* Clipped policy loss: ratio = exp(log p(action) - logp_old),
  *   loss = w (-min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coeff kl - entropy_coeff H),
  *   kl = exp(d) - d - 1 with d = logp_ref - log p(action).
- * logp_ref may be NULL where kl_coeff is 0 (kl is 0 then). */
+ * A term whose coefficient is 0, or whose advantage A is 0, is none, however large its other factor. logp_ref may be NULL
+ * where kl_coeff is 0 (kl is 0 then); given all the same, kl is reported. */
 typedef struct {
     const int32_t *actions;                     /* [rows] */
     const float *logp_old, *advantages;         /* [rows] */
@@ -276,10 +279,10 @@ int sk_policy_loss(sk_ctx *ctx, const sk_logits *logits, const sk_policy *policy
  * margin = beta h - target_margin, and with e = label_smoothing
  *   SIGMOID  loss = w (-(1 - e) log sigmoid(margin) - e log sigmoid(-margin))
  *   HINGE    loss = w max(0, 1 - margin)
- *   SQUARED  loss = w (margin - 1/2)^2
+ *   SQUARED  loss = w (margin - 1/2)^2: beta^2 times (h - 1 / (2 beta))^2 where target_margin is 0
  * Rows below offsets[0] and from offsets[2 pairs] on belong to no sequence: log-probability and gradient zero. Offsets
  * that fall, or leave [0, rows], make their sequence an empty one and are reported by the next sk_sync; rows that then
- * belong to sequences of several pairs get the sum of their gradients. */
+ * belong to sequences of several pairs get the sum of their gradients, added in any order. */
 typedef struct {
     const int32_t *labels;          /* [rows] */
     const int32_t *offsets;         /* [2 pairs + 1] */

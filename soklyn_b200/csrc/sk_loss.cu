@@ -111,8 +111,9 @@ template <typename T> cudaError_t sequence_gradient_impl(sk_ctx *c, const loss::
 template <typename T> cudaError_t distill_impl(sk_ctx *c, const loss::Rows &r, const loss::Distill &op) {
     RowPlan plan = plan_row(c, r, sizeof(T), r.d != nullptr);
     const uint32_t threads = std::max(plan.threads, 64u);
-    // A block has 48 KB without asking for more, and a row's bits may take 128: more blocks share such a row (four at 2^20 classes)
-    // rather than one block keeping an SM to itself. A gradient's rows are shared by enough blocks for other reasons.
+    // A block has 48 KB without asking for more, and a row's bits may take 128: more blocks share such a row (four at 2^20 classes).
+    // One block with up to 128 KB leaves an SM one or two of them: 1000 bf16 rows of 2^20 classes took 1035 us against 421,
+    // 80 rows 149 against 57, 1000 rows of 400000 210 against 172. A gradient's rows are shared by enough blocks for other reasons.
     constexpr size_t room = 48 * 1024 - sizeof(loss::DistillShared<kMostThreads>);
     while (plan.ranks < loss::kMaxCluster && loss::bit_bytes<T>(r.classes, plan.ranks) > room) plan.ranks *= 2;
     static_assert(loss::kMaxListClasses / loss::kMaxCluster / 8 + 64 <= room, "the bits of the widest row fit the blocks of a cluster");
